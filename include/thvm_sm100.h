@@ -713,6 +713,110 @@ int sm100_attn_prefill_bf16(const void *q, const void *k, const void *v, float *
  * synchronises the device and clears the word */
 uint32_t sm100_attn_prefill_status(void);
 
+/* ---- paged key / value cache ------------------------------------------------ */
+/* Keys and values of many sequences in pages of `page` tokens, so that a
+ * sequence holds the pages that its length needs and no fixed slot.  pool is
+ * uint8 [n_pages][kv_heads][block], block = sm100_paged_block_bytes: the keys
+ * and then the values of the page's tokens, each
+ *   SM100_KV_BF16  bf16 [page][head_dim]
+ *   SM100_KV_Q4    codes [page][head_dim / 2] (dimension 2 i in the low half of
+ *                  byte i, 2 i + 1 in the high half), then bf16 (scale,
+ *                  minimum) pairs [page][head_dim / 64][2]: a code c of a group
+ *                  of 64 dimensions stands for minimum + c * scale
+ * (a page and head is one contiguous block, so attention brings it in by one
+ * bulk copy).  table [n_seq][max_pages] (device) is the page of each page slot
+ * of a sequence: token p of sequence s is row p % page of page
+ * table[s][p / page].  page 16, 32 or 64; head_dim 64, 128 or 256; pool
+ * 16-byte aligned. */
+enum { SM100_KV_Q4 = 4, SM100_KV_BF16 = 16 };
+typedef struct Sm100PagedCache {
+  void *pool;
+  const int32_t *table;
+  int32_t n_pages, page, kv_heads, head_dim, bits, n_seq, max_pages;
+} Sm100PagedCache;
+uint64_t sm100_paged_block_bytes(int32_t page, int32_t head_dim, int32_t bits); /* 0: no such layout */
+/* T rows of a fused projection (row t: q [heads] | k [kv_heads] | v [kv_heads]
+ * heads of head_dim, f32 or bf16, row stride ld elements) at position pos[t]
+ * of sequence seq[t]: with g_q / g_k (f32 [head_dim], or NULL) each query /
+ * key head becomes y = x * rsqrt(mean(x^2) + eps) * g; with cos_t / sin_t (f32
+ * [n_pos][rot / 2], or NULL) the first rot dimensions of each query and key
+ * head are rotated by row pos[t] (pair i: dimensions i and i + rot / 2, or
+ * with pairs != 0 dimensions 2 i and 2 i + 1); queries go to q_out (bf16 [T]
+ * [heads][head_dim]), keys and values into the cache.  All in f32, rounded
+ * once (Q4: to codes of the group's bf16 scale = (max - min) / 15 and minimum;
+ * a group with a value that is not finite reads as NaN).  A row whose
+ * sequence, position or page is outside the cache or the tables is skipped:
+ * its queries are zeros and sm100_paged_status gets SM100_DECODE_ERR_ARG.  No
+ * two rows of a call may be the same token.  qkv, q_out 16-byte aligned, ld a
+ * multiple of 8 (bf16) or 4 (f32), rot a multiple of 16. */
+typedef struct Sm100PagedAppendArgs {
+  const void *qkv;
+  const float *g_q, *g_k, *cos_t, *sin_t;
+  const int32_t *pos, *seq;
+  void *q_out;
+  int64_t ld; /* 0: dense */
+  int32_t T, heads, dtype /* SM100_DT_F32 or SM100_DT_BF16 */, rot, n_pos, pairs;
+  float eps;
+} Sm100PagedAppendArgs;
+int sm100_paged_append(const Sm100PagedCache *c, const Sm100PagedAppendArgs *a, void *stream);
+/* k, v (bf16 [T][kv_heads][head_dim]) = the values that the cache holds for
+ * token pos[t] of sequence seq[t] (zeros, and the status word, outside it) */
+int sm100_paged_read(const Sm100PagedCache *c, const int32_t *pos, const int32_t *seq, void *k, void *v, int32_t T,
+                     void *stream);
+/* out (bf16 [T][heads][head_dim]) = softmax(q k^T * scale) v over the cache,
+ * query head h reading key head h / (heads / kv_heads).  Sequence s has the
+ * rows q_off[s] .. q_off[s + 1] - 1 (q_off NULL: row s alone, T = n_seq), at
+ * most max_rows of them, at its last positions: of n rows, row r sees keys
+ * 0 .. kv_len[s] - n + r (kv_len counts the new tokens, appended before).  A
+ * row that sees none (an idle sequence: kv_len 0) is zeros.  Tokens whose page
+ * is outside the pool are left out and set the status word, as does a length
+ * past max_pages * page (cut there).  q bf16, row stride ld_q elements (0:
+ * dense), a multiple of 8; q, out, ws 16-byte aligned; heads / kv_heads whole.
+ * ws: sm100_paged_attention_ws_bytes of scratch, zeroed before its first use and
+ * left ready for the next call; calls that can overlap on the GPU need one
+ * each. */
+typedef struct Sm100PagedAttnArgs {
+  const void *q;
+  const int32_t *kv_len, *q_off;
+  void *out, *ws;
+  uint64_t ws_bytes;
+  int64_t ld_q;
+  int32_t T, heads, max_rows;
+  float scale;
+} Sm100PagedAttnArgs;
+int sm100_paged_attention(const Sm100PagedCache *c, const Sm100PagedAttnArgs *a, void *stream);
+uint64_t sm100_paged_attention_ws_bytes(const Sm100PagedCache *c, int32_t heads, int32_t max_rows);
+/* the sticky status of the paged calls (SM100_DECODE_ERR_*); synchronises the
+ * device and clears the word */
+uint32_t sm100_paged_status(void);
+
+/* ---- the next ids from logits ------------------------------------------------- */
+/* Row b of logits (f32 or bf16 [B][V], row stride ld) in the order of falling
+ * logit, equal ones by rising id; d_i = (l_i - l_max) / temperature[b], w_i =
+ * exp(d_i).  Kept are: the first top_k[b] ids (<= 0: all); of those, the ids
+ * whose forerunners hold less than top_p[b] of their weight (>= 1: all); of
+ * those, the ids with w_i >= min_p[b]; always the first id.  tok[b] is the kept
+ * id with the largest d_i - ln(noise_i) (equal ones: the lowest id): with
+ * noise (f32 [B][V], row stride ld_noise) drawn from the unit exponential
+ * distribution an id is chosen with probability w_i / (the kept weight), whose
+ * logarithm is logp[b] (f32, or NULL).  temperature[b] <= 0 takes the first id
+ * (logp 0).  Logits of -inf or NaN are left out, +inf counts as the largest
+ * float; a row with none left gives id -1 and logp -inf.  temperature, top_k,
+ * top_p, min_p: device arrays [B], or NULL (1, all, all, all).  V < 2^23.  The
+ * weights of the filters are summed exactly in units of 2^-40: the cut does
+ * not depend on an order of summation. */
+typedef struct Sm100SampleArgs {
+  const void *logits;
+  const float *noise, *temperature;
+  const int32_t *top_k;
+  const float *top_p, *min_p;
+  int32_t *tok;
+  float *logp;
+  int64_t ld, ld_noise; /* 0: V */
+  int32_t B, V, dtype;  /* SM100_DT_F32 or SM100_DT_BF16 */
+} Sm100SampleArgs;
+int sm100_sample(const Sm100SampleArgs *a, void *stream);
+
 /* ---- weight files straight into device buffers ---------------------------
  * .safetensors (the format py/thvm/nn_state.py safe_load / safe_save read
  * and write, :44-85: an 8-byte little-endian header length, a JSON header of

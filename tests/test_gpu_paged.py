@@ -1,0 +1,438 @@
+"""The paged key / value cache (thvm_b200.paged): append with per-head norms
+and rotation, reading back, and attention, against the formulas in 64 bits.
+
+Tolerances, from the roundings that the operators state:
+  bf16 values     one rounding to 8 significant bits (2^-8 of the value, half a
+                  unit) of an f32 result whose own error is a few 2^-24 of the
+                  largest term (2^-18 of the head's largest value)
+  4-bit values    half a step s, plus the rounding of s (15 s 2^-8) and of the
+                  minimum (2^-8 of it) to bf16, plus the bf16 value read back
+  attention       each weight enters the second product rounded to at least 8
+                  bits: 2^-8 of sum p |v|; logits in f32 (2^-12 of it is ample);
+                  one rounding of the output
+"""
+import ctypes
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+GROUP = 64
+
+
+def _table(lengths, page, rng, max_pages=None, spare=3):
+    """A shuffled page table for sequences of these lengths; returns (table, n_pages)."""
+    import torch
+    need = [-(-n // page) for n in lengths]
+    total = sum(need) + spare
+    ids = rng.permutation(total)
+    t = np.full((len(lengths), max_pages or max(max(need), 1)), -1, np.int32)
+    at = 0
+    for s, n in enumerate(need):
+        t[s, :n] = ids[at:at + n]
+        at += n
+    return torch.from_numpy(t).cuda(), total
+
+
+def _cache(lengths, kv, hd, page, bits, rng, **kw):
+    import torch
+    from thvm_b200.paged import PagedCache
+    table, total = _table(lengths, page, rng, **kw)
+    c = PagedCache.empty(len(lengths), table.shape[1], total, kv, hd, page, bits)
+    c.table.copy_(table)
+    # rows that no call has written hold whatever was there: NaN patterns, which must never reach a result
+    c.pool.copy_(torch.full_like(c.pool, 0xFF))
+    return c
+
+
+def _unpack(c):
+    """The pool by its documented layout: values f64 [n_pages, kv, 2, page, hd], (scale, minimum) f64 in 4 bits."""
+    import torch
+    n, kv, _ = c.pool.shape
+    page, hd = c.page, c.head_dim
+    x = c.pool.view(n, kv, 2, -1)
+    if c.bits == 16:
+        return x.contiguous().view(torch.bfloat16).double().view(n, kv, 2, page, hd), None
+    codes = x[..., :page * hd // 2].reshape(n, kv, 2, page, hd // 2)
+    marks = x[..., page * hd // 2:].contiguous().view(torch.bfloat16).double().view(n, kv, 2, page, hd // GROUP, 2)
+    code = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).double()
+    s, m = (marks[..., i].repeat_interleave(GROUP, -1) for i in (0, 1))
+    return m + code * s, marks
+
+
+def _rows(c, pos, seq):
+    """Values (and scales) of token pos[t] of sequence seq[t], [T, kv, 2, hd]."""
+    v, marks = _unpack(c)
+    at = c.table[seq.long(), (pos // c.page).long()].long()
+    r = (pos % c.page).long()
+    return v[at, :, :, r], None if marks is None else marks[at, :, :, r]
+
+
+def _tables(n, rot):
+    import torch
+    a = torch.arange(n, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(rot // 2, dtype=torch.float64) * 2 / rot)
+    return a.cos().float().cuda(), a.sin().float().cuda()
+
+
+def _want(qkv, pos, H, kv, hd, g_q, g_k, cos, sin, pairs, eps):
+    """q, k, v in f64 by the formulas."""
+    import torch
+    x = qkv.double().view(len(qkv), -1, hd)
+    out = [x[:, :H], x[:, H:H + kv], x[:, H + kv:]]
+    for i, g in ((0, g_q), (1, g_k)):
+        if g is not None:
+            out[i] = out[i] / torch.sqrt((out[i] ** 2).mean(-1, keepdim=True) + eps) * g.double()
+        if cos is not None:
+            half = cos.shape[1]
+            j = torch.arange(half, device=x.device)
+            a, b = (2 * j, 2 * j + 1) if pairs else (j, j + half)
+            cc, ss = (t.double()[pos.long()][:, None] for t in (cos, sin))
+            y = out[i].clone()
+            y[..., a], y[..., b] = out[i][..., a] * cc - out[i][..., b] * ss, out[i][..., b] * cc + out[i][..., a] * ss
+            out[i] = y
+    return out
+
+
+def _near(got, want, rel=2.0 ** -8):
+    err = (got.double() - want).abs()
+    tol = rel * want.abs() + 2.0 ** -18 * want.abs().amax(-1, keepdim=True)
+    assert bool((err <= tol).all()), float((err - tol).max())
+
+
+APPEND = [
+    # heads, kv, hd, page, rows per sequence, starts, norm, rot, pairs, f32
+    (1, 1, 64, 16, [1], [0], False, 0, False, True),
+    (12, 12, 64, 16, [1], [15], True, 64, False, False),
+    (4, 1, 64, 32, [5, 1, 33], [0, 31, 16], True, 32, True, True),
+    (7, 7, 64, 16, [3, 18], [14, 1], False, 16, False, False),
+    (8, 2, 128, 64, [1] * 9, [0, 63, 64, 65, 127, 128, 1, 2, 500], True, 128, False, True),
+    (28, 4, 128, 32, [37, 64], [3, 0], True, 64, True, False),
+    (5, 5, 128, 16, [129], [7], False, 128, True, True),
+    (16, 2, 256, 16, [21, 2], [11, 30], True, 256, False, False),
+    (3, 1, 256, 64, [70], [60], True, 48, False, True),
+]
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("case", APPEND, ids=lambda c: f"{c[0]}x{c[1]}x{c[2]}p{c[3]}r{c[7]}")
+def test_append_matches_the_formulas(case, bits):
+    import torch
+    H, kv, hd, page, new, start, norm, rot, pairs, f32 = case
+    rng = np.random.default_rng(hd + sum(new) + bits)
+    c = _cache([a + n for a, n in zip(start, new)], kv, hd, page, bits, rng)
+    before = c.pool.clone()
+    pos = torch.cat([torch.arange(a, a + n) for a, n in zip(start, new)]).int().cuda()
+    seq = torch.arange(len(new)).repeat_interleave(torch.tensor(new)).int().cuda()
+    T, width = len(pos), (H + 2 * kv) * hd
+    order = torch.from_numpy(rng.permutation(T)).cuda()   # rows come in any order
+    pos, seq = pos[order].contiguous(), seq[order].contiguous()
+    x = torch.from_numpy(rng.standard_normal((T, width + 16)).astype(np.float32) * 2).cuda()
+    x = (x if f32 else x.bfloat16())[:, 8:8 + width]      # strided rows
+    g = [torch.from_numpy(rng.uniform(0.5, 1.5, hd).astype(np.float32)).cuda() for _ in range(2)] if norm else [None] * 2
+    cos, sin = _tables(700, rot) if rot else (None, None)
+    q = c.append(x, pos, seq, H, *g, cos, sin, pairs, eps=1e-5)
+    wq, wk, wv = _want(x, pos, H, kv, hd, *g, cos, sin, pairs, 1e-5)
+    _near(q, wq)
+    got, marks = _rows(c, pos, seq)
+    want = torch.stack((wk, wv), 2)
+    if bits == 16:
+        _near(got, want)
+    else:
+        y = want.unflatten(-1, (-1, GROUP))
+        lo, hi = y.amin(-1), y.amax(-1)
+        step = ((hi - lo) / 15).repeat_interleave(GROUP, -1)
+        lo = lo.abs().repeat_interleave(GROUP, -1)
+        assert bool(((got - want).abs() <= (0.5 + 15 * 2.0 ** -8) * step + 2.0 ** -8 * lo + 1e-5).all())
+    k, v = c.read(pos, seq)
+    assert torch.equal(k, got[:, :, 0].float().bfloat16()) and torch.equal(v, got[:, :, 1].float().bfloat16())
+    # nothing but the rows' own bytes changed
+    n, token = c.pool.shape[0], 2 * hd if bits == 16 else hd // 2
+    touched = torch.zeros(n, page, dtype=torch.bool, device="cuda")
+    touched[c.table[seq.long(), (pos // page).long()].long(), (pos % page).long()] = True
+    a, b = (t.view(n, kv, 2, -1)[..., :page * token].view(n, kv, 2, page, token) for t in (before, c.pool))
+    assert bool((a == b).all(-1).all(2).all(1)[~touched].all())
+    assert c.status() == 0
+
+
+def test_append_skips_rows_outside_the_cache_and_keeps_nan_visible():
+    import torch
+    from thvm_b200 import _lib as L
+    rng = np.random.default_rng(3)
+    c = _cache([40, 20], 2, 64, 16, 4, rng, max_pages=4)
+    before = c.pool.clone()
+    pos = torch.tensor([5, 64, -1, 3, 48, 9], dtype=torch.int32).cuda()   # 64: past the table; 48: an empty slot
+    seq = torch.tensor([0, 0, 0, 2, 0, -1], dtype=torch.int32).cuda()
+    x = torch.randn(6, 6 * 64).cuda()
+    x[0, 2 * 64 + 7] = float("nan")    # key head 0
+    x[0, 4 * 64 + 9] = float("inf")    # value head 0
+    q = c.append(x, pos, seq, 2)
+    assert c.status() == L.DECODE_ERR_ARG
+    assert c.status() == 0             # read once
+    assert bool((q[1:] == 0).all()) and bool((q[0] != 0).any())
+    k, v = c.read(pos[:1].contiguous(), seq[:1].contiguous())
+    assert bool(torch.isnan(k[0, 0]).all()) and bool(torch.isnan(v[0, 0]).all())
+    assert bool(torch.isfinite(k[0, 1]).all()) and bool(torch.isfinite(v[0, 1]).all())
+    page = int(c.table[0, 0])
+    same = (c.pool == before).all(-1).all(-1)
+    assert bool(same[torch.arange(len(same)) != page].all())
+    k, v = c.read(pos, seq)
+    assert bool((k[1:] == 0).all()) and bool((v[1:] == 0).all())
+    assert c.status() == L.DECODE_ERR_ARG
+    # past the rotation tables
+    cos, sin = _tables(5, 64)
+    q = c.append(x[:1], pos[:1].contiguous(), seq[:1].contiguous(), 2, cos=cos, sin=sin)
+    assert c.status() == L.DECODE_ERR_ARG and bool((q == 0).all())
+    assert c.append(x[:0], pos[:0], seq[:0], 2).shape == (0, 2, 64)
+
+
+def test_append_constant_groups_and_offsets():
+    """A constant group reads as its (bf16) value; a far offset costs its bf16 rounding and no more."""
+    import torch
+    rng = np.random.default_rng(4)
+    c = _cache([3], 1, 64, 16, 4, rng)
+    x = torch.zeros(3, 3 * 64).cuda()
+    x[0, 64:128] = 1.7
+    x[1, 64:128] = 100 + torch.rand(64).cuda()
+    x[2, 128:192] = 1e-30 * torch.randn(64).cuda()
+    pos, seq = torch.arange(3).int().cuda(), torch.zeros(3).int().cuda()
+    c.append(x, pos, seq, 1)
+    k, v = c.read(pos, seq)
+    assert bool((k[0] == torch.tensor(1.7).bfloat16().cuda()).all())
+    assert float((k[1].float() - x[1, 64:128]).abs().max()) <= 0.5 + 0.5 / 15 + 0.25   # m and the value read, in bf16
+    want = x[2, 128:192]
+    assert float((v[2, 0].float() - want).abs().max()) <= (0.6 / 15 + 2.0 ** -7) * float(want.max() - want.min())
+    assert c.status() == 0
+
+
+ATTEND = [
+    # heads, kv, hd, page, lengths, rows per sequence
+    (1, 1, 64, 16, [1], [1]),
+    (12, 12, 64, 16, [37], [1]),
+    (25, 25, 64, 16, [1, 15, 16, 17, 300], [1] * 5),
+    (8, 1, 64, 32, [64, 0, 63, 65, 1000], [1] * 5),
+    (32, 8, 128, 64, [2500, 1, 129, 0, 64], [1] * 5),
+    (28, 4, 128, 32, [5000], [1]),
+    (16, 16, 128, 16, [130, 255], [1, 1]),
+    (64, 8, 128, 64, [100, 7, 513], [4, 4, 2]),
+    (6, 2, 128, 16, [40, 3, 200], [5, 7, 0]),      # more rows than tokens: the first see none
+    (8, 8, 128, 16, [90, 33], [33, 33]),
+    (40, 1, 64, 16, [77, 500], [1, 3]),            # 40 query heads on one key head
+    (16, 2, 256, 16, [300, 17], [1, 1]),
+    (5, 1, 256, 64, [200, 64], [9, 2]),
+    (4, 4, 64, 32, [3] * 70, [1] * 70),
+]
+
+
+def _fill(c, lens, rng, spread=1.0):
+    """Random keys and values through append, with a few strong key channels."""
+    import torch
+    pos = torch.cat([torch.arange(n) for n in lens]).int().cuda()
+    seq = torch.arange(len(lens)).repeat_interleave(torch.tensor(lens)).int().cuda()
+    x = torch.from_numpy(rng.standard_normal((len(pos), 3 * c.kv_heads * c.head_dim)).astype(np.float32)).cuda() * spread
+    x[:, c.kv_heads * c.head_dim::37] *= 3
+    if len(pos):
+        c.append(x, pos, seq, c.kv_heads)
+
+
+def _attend_want(c, q, lens, rows, scale):
+    """(out, sum p |v|) in f64 from the values that the cache holds."""
+    import torch
+    values, _ = _unpack(c)
+    H, G = q.shape[1], q.shape[1] // c.kv_heads
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    size = torch.zeros_like(out)
+    at = 0
+    for s, (n, r) in enumerate(zip(lens, rows)):
+        if n:
+            pages = c.table[s, :-(-n // c.page)].long()
+            x = values[pages].permute(0, 3, 2, 1, 4).reshape(-1, 2, c.kv_heads, c.head_dim)[:n]
+            for i in range(r):
+                m = n - r + i + 1
+                if m <= 0:
+                    continue
+                qi = q[at + i].double().view(c.kv_heads, G, -1)
+                p = torch.softmax(torch.einsum("kgd,nkd->kgn", qi, x[:m, 0]) * scale, -1)
+                out[at + i] = torch.einsum("kgn,nkd->kgd", p, x[:m, 1]).reshape(H, -1)
+                size[at + i] = torch.einsum("kgn,nkd->kgd", p, x[:m, 1].abs()).reshape(H, -1)
+        at += r
+    return out, size
+
+
+def _check_attention(got, want, size):
+    err = (got.double() - want).abs()
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * size + 1e-30
+    assert bool((err <= tol).all()), float((err - tol).max())
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("case", ATTEND, ids=lambda c: f"{c[0]}x{c[1]}x{c[2]}p{c[3]}n{len(c[4])}x{max(c[5])}")
+def test_attention_matches_the_formula(case, bits):
+    import torch
+    H, kv, hd, page, lens, rows = case
+    rng = np.random.default_rng(H + hd + sum(lens) + bits)
+    c = _cache(lens, kv, hd, page, bits, rng)
+    _fill(c, lens, rng)
+    T = sum(rows)
+    wide = torch.from_numpy(rng.standard_normal((T, H * hd + 24)).astype(np.float32)).cuda().bfloat16()
+    q = wide[:, 8:8 + H * hd].unflatten(1, (H, hd))       # strided rows
+    kv_len = torch.tensor(lens, dtype=torch.int32).cuda()
+    ragged = rows != [1] * len(lens)
+    q_off = torch.tensor(np.concatenate([[0], np.cumsum(rows)]), dtype=torch.int32).cuda()
+    want, size = _attend_want(c, q, lens, rows, hd ** -0.5)
+    for _ in range(2):   # the scratch is left ready for the next call
+        got = c.attend(q, kv_len, q_off=q_off if ragged else None, max_rows=max(rows))
+        _check_attention(got, want, size)
+    if not ragged:       # the same rows by offsets, and with room for more rows than there are
+        _check_attention(c.attend(q, kv_len, q_off=q_off, max_rows=3), want, size)
+    assert c.status() == 0
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_attention_of_strong_logits_and_small_values(bits):
+    """Logits in the hundreds (a softmax that is one key), tiny and huge values."""
+    import torch
+    rng = np.random.default_rng(11)
+    lens = [700, 65]
+    for spread in (12.0, 1e-6, 1e4):
+        c = _cache(lens, 2, 128, 32, bits, rng)
+        _fill(c, lens, rng, spread)
+        q = torch.from_numpy(rng.standard_normal((2, 8, 128)).astype(np.float32)).cuda().bfloat16()
+        kv_len = torch.tensor(lens, dtype=torch.int32).cuda()
+        scale = 0.5 if spread > 1 else 1.0
+        if spread == 1e4:
+            q *= 1e-3
+        want, size = _attend_want(c, q, lens, [1, 1], scale)
+        got = c.attend(q, kv_len, scale=scale)
+        err = (got.double() - want).abs()
+        # logits of size z come with an f32 error of up to 2^-20 z, each weight with that much more
+        z = float(12.0 * 128 * 0.5 * 9 if spread == 12.0 else 64)
+        assert bool((err <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12 + 2.0 ** -20 * z) * size).all())
+        assert c.status() == 0
+
+
+def test_attention_leaves_out_pages_outside_the_pool():
+    """A bad page id: its tokens are left out of the softmax, the status says so; a length past the table is cut."""
+    import torch
+    from thvm_b200 import _lib as L
+    rng = np.random.default_rng(5)
+    for bits in (4, 16):
+        c = _cache([200, 48], 2, 64, 16, bits, rng)
+        _fill(c, [200, 48], rng)
+        q = torch.from_numpy(rng.standard_normal((2, 4, 64)).astype(np.float32)).cuda().bfloat16()
+        kv_len = torch.tensor([200, 48], dtype=torch.int32).cuda()
+        full, _ = _attend_want(c, q, [200, 48], [1, 1], 0.125)
+        assert c.status() == 0
+        c.table[0, 2:4] = torch.tensor([-1, 10 ** 6], dtype=torch.int32).cuda()
+        got = c.attend(q, kv_len)
+        assert c.status() == L.DECODE_ERR_ARG
+        keep = torch.tensor([i for i in range(200) if not 32 <= i < 64]).cuda()
+        values, _ = _unpack(c)
+        pages = c.table[0, :13].long().clamp(0, c.pool.shape[0] - 1)
+        x = values[pages].permute(0, 3, 2, 1, 4).reshape(-1, 2, 2, 64)[keep]
+        p = torch.softmax(torch.einsum("kgd,nkd->kgn", q[0].double().view(2, 2, 64), x[:, 0]) * 0.125, -1)
+        o = torch.einsum("kgn,nkd->kgd", p, x[:, 1]).reshape(4, 64)
+        size = torch.einsum("kgn,nkd->kgd", p, x[:, 1].abs()).reshape(4, 64)
+        _check_attention(got[0], o, size)
+        _check_attention(got[1:], full[1:], torch.full_like(full[1:], 8.0))
+        # every page of a row gone: zeros
+        c.table[1, :3] = -1
+        got = c.attend(q, kv_len)
+        assert bool((got[1] == 0).all()) and c.status() == L.DECODE_ERR_ARG
+        c.attend(q, torch.tensor([10 ** 6, 0], dtype=torch.int32).cuda())
+        assert c.status() == L.DECODE_ERR_ARG
+
+
+def test_attention_offsets_past_two_gigabytes():
+    """A pool of 5 GB whose used pages lie at its far end."""
+    import torch
+    from thvm_b200.paged import PagedCache
+    rng = np.random.default_rng(6)
+    kv, hd, page = 8, 128, 64
+    n_pages = 5 * (1 << 30) // (kv * 4 * page * hd)
+    c = PagedCache.empty(1, 4, n_pages, kv, hd, page, 16)
+    c.table.copy_(torch.tensor([[n_pages - 1, n_pages // 2, n_pages - 2, 1]], dtype=torch.int32))
+    pos, seq = torch.arange(200).int().cuda(), torch.zeros(200).int().cuda()
+    x = torch.from_numpy(rng.standard_normal((200, 3 * kv * hd)).astype(np.float32)).cuda()
+    c.append(x, pos, seq, kv)
+    k, v = c.read(pos, seq)
+    assert torch.equal(k, x[:, kv * hd:2 * kv * hd].bfloat16().view(200, kv, hd))
+    assert torch.equal(v, x[:, 2 * kv * hd:].bfloat16().view(200, kv, hd))
+    q = torch.from_numpy(rng.standard_normal((1, 16, hd)).astype(np.float32)).cuda().bfloat16()
+    got = c.attend(q, torch.tensor([200], dtype=torch.int32).cuda())
+    p = torch.softmax(torch.einsum("kgd,nkd->kgn", q[0].double().view(kv, 2, hd), k.double()) * hd ** -0.5, -1)
+    _check_attention(got[0], torch.einsum("kgn,nkd->kgd", p, v.double()).reshape(16, hd),
+                     torch.einsum("kgn,nkd->kgd", p, v.double().abs()).reshape(16, hd))
+    assert c.status() == 0
+
+
+def test_paged_calls_on_another_stream_and_in_a_graph():
+    """append and attend captured into one graph on a side stream: replays follow the device positions."""
+    import torch
+    rng = np.random.default_rng(8)
+    H, kv, hd, page = 8, 2, 128, 16
+    c = _cache([100, 100], kv, hd, page, 4, rng)
+    _fill(c, [60, 33], rng)
+    kv_len = torch.tensor([61, 34], dtype=torch.int32).cuda()
+    pos, seq = kv_len - 1, torch.arange(2).int().cuda()
+    x = torch.from_numpy(rng.standard_normal((2, (H + 2 * kv) * hd)).astype(np.float32)).cuda()
+    q, o = (torch.empty(2, H, hd, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c.append(x, pos, seq, H, out=q)
+        c.attend(q, kv_len, out=o)
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.append(x, pos, seq, H, out=q)
+        c.attend(q, kv_len, out=o)
+    for step in range(20):
+        x.copy_(torch.from_numpy(rng.standard_normal(x.shape).astype(np.float32)))
+        g.replay()
+        want, size = _attend_want(c, q, [61 + step, 34 + step], [1, 1], hd ** -0.5)
+        _check_attention(o, want, size)
+        pos += 1
+        kv_len += 1
+    assert c.status() == 0
+
+
+def test_refusals():
+    import torch
+    from thvm_b200 import _lib as L
+    from thvm_b200.paged import PagedCache
+    c = PagedCache.empty(2, 2, 4, 2, 64, 16, 16)
+    i = lambda *v: torch.tensor(v, dtype=torch.int32).cuda()
+    x = torch.zeros(1, 6 * 64).cuda()
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError):
+        PagedCache.empty(2, 2, 4, 2, 96, 16, 16)
+    with pytest.raises(ValueError):
+        PagedCache(c.pool, c.table.long(), 16, 64, 16)
+    with pytest.raises(ValueError):
+        c.append(x[:, :64], i(0), i(0), 2)
+    with pytest.raises(ValueError):
+        c.append(x.half(), i(0), i(0), 2)
+    with pytest.raises(ValueError):
+        c.append(x, i(0, 1), i(0), 2)
+    with pytest.raises(ValueError):
+        c.append(x, i(0), i(0), 2, cos=torch.zeros(4, 32).cuda())
+    with pytest.raises(ValueError):
+        c.append(x.expand(3, -1), i(0, 1, 2), i(0, 0, 0), 2)
+    with pytest.raises(L.Sm100Error):   # rot 24
+        c.append(x, i(0), i(0), 2, cos=torch.zeros(4, 12).cuda(), sin=torch.zeros(4, 12).cuda())
+    with pytest.raises(L.Sm100Error):   # rows that do not start on 16 bytes
+        c.append(torch.zeros(2, 6 * 64 + 1).cuda()[:, 1:], i(0, 1), i(0, 0), 2)
+    with pytest.raises(ValueError):
+        c.attend(q.float(), i(1, 1))
+    with pytest.raises(ValueError):
+        c.attend(q, i(1))
+    with pytest.raises(ValueError):
+        c.attend(torch.zeros(2, 3, 64, dtype=torch.bfloat16, device="cuda"), i(1, 1))   # 3 heads on 2
+    with pytest.raises(L.Sm100Error):
+        c.attend(q[:1], i(1, 1))        # one row for two sequences, no offsets
+    assert c.attend(q[:0], i(0, 0), q_off=i(0, 0, 0)).shape == (0, 4, 64)
+    small = L.Sm100PagedAttnArgs(q.data_ptr(), c.table.data_ptr(), None, q.data_ptr(), q.data_ptr(), 0, 0, 2, 4, 1, 1.0)
+    assert L.lib().sm100_paged_attention(c._desc, ctypes.byref(small), None) == L.ERR_ARG
+    assert b"scratch" in L.lib().sm100_last_error()
+    assert c.status() == 0

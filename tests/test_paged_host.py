@@ -1,0 +1,93 @@
+"""Argument checks of the paged cache and the sampler, on the CPU: calls outside
+their contracts come back with a status and a message before anything touches
+a device."""
+import ctypes
+
+from thvm_b200 import _lib as L
+
+P = 1 << 20   # an aligned stand-in address; never dereferenced
+
+
+def _cache(**kw):
+    a = dict(pool=P, table=P, n_pages=4, page=16, kv_heads=2, head_dim=64, bits=16, n_seq=2, max_pages=2) | kw
+    return L.Sm100PagedCache(*(a[n] for n, _ in L.Sm100PagedCache._fields_))
+
+
+def _append(c, **kw):
+    a = dict(qkv=P, g_q=P, g_k=P, cos_t=P, sin_t=P, pos=P, seq=P, q_out=P, ld=0, T=1, heads=4, dtype=L.DT_F32, rot=64,
+             n_pos=8, pairs=0, eps=1e-6) | kw
+    a = L.Sm100PagedAppendArgs(*(a[n] for n, _ in L.Sm100PagedAppendArgs._fields_))
+    return L.lib().sm100_paged_append(ctypes.byref(c), ctypes.byref(a), None)
+
+
+def _attend(c, **kw):
+    a = dict(q=P, kv_len=P, q_off=P, out=P, ws=P, ws_bytes=1 << 40, ld_q=0, T=2, heads=4, max_rows=1, scale=1.0) | kw
+    a = L.Sm100PagedAttnArgs(*(a[n] for n, _ in L.Sm100PagedAttnArgs._fields_))
+    return L.lib().sm100_paged_attention(ctypes.byref(c), ctypes.byref(a), None)
+
+
+def _sample(**kw):
+    a = dict(logits=P, noise=P, temperature=None, top_k=None, top_p=None, min_p=None, tok=P, logp=None, ld=0,
+             ld_noise=0, B=1, V=8, dtype=L.DT_F32) | kw
+    a = L.Sm100SampleArgs(*(a[n] for n, _ in L.Sm100SampleArgs._fields_))
+    return L.lib().sm100_sample(ctypes.byref(a), None)
+
+
+def test_struct_layouts():
+    assert ctypes.sizeof(L.Sm100PagedCache) == 48
+    assert ctypes.sizeof(L.Sm100PagedAppendArgs) == 104 and L.Sm100PagedAppendArgs.ld.offset == 64
+    assert ctypes.sizeof(L.Sm100PagedAttnArgs) == 72 and L.Sm100PagedAttnArgs.T.offset == 56
+    assert ctypes.sizeof(L.Sm100SampleArgs) == 96 and L.Sm100SampleArgs.B.offset == 80
+
+
+def test_block_bytes():
+    f = L.lib().sm100_paged_block_bytes
+    assert f(16, 64, 16) == 2 * 16 * 64 * 2
+    assert f(32, 128, 4) == 2 * 32 * (64 + 8)
+    assert f(64, 256, 4) == 2 * 64 * (128 + 16)
+    for bad in ((8, 64, 16), (48, 64, 16), (16, 96, 4), (16, 64, 8), (0, 0, 0), (-16, 64, 4)):
+        assert f(*bad) == 0
+
+
+def test_cache_refusals():
+    for bad in (dict(pool=None), dict(table=None), dict(pool=P + 8), dict(n_pages=0), dict(kv_heads=0), dict(n_seq=0),
+                dict(max_pages=0), dict(max_pages=1 << 28)):
+        c = _cache(**bad)
+        assert _append(c) == _attend(c) == L.ERR_ARG, bad
+        assert L.lib().sm100_paged_read(ctypes.byref(c), P, P, P, P, 1, None) == L.ERR_ARG
+        assert L.lib().sm100_paged_attention_ws_bytes(ctypes.byref(c), 4, 1) == 0
+    for bad in (dict(page=8), dict(head_dim=96), dict(bits=8)):
+        c = _cache(**bad)
+        assert _append(c) == _attend(c) == L.ERR_UNSUPPORTED, bad
+        assert b"head_dim" in L.lib().sm100_last_error()
+
+
+def test_append_refusals():
+    c = _cache()
+    for bad in (dict(qkv=None), dict(pos=None), dict(seq=None), dict(q_out=None), dict(T=-1), dict(heads=0),
+                dict(heads=3), dict(qkv=P + 4), dict(q_out=P + 2), dict(g_q=P + 4), dict(cos_t=None), dict(sin_t=None),
+                dict(sin_t=P + 4), dict(rot=0), dict(rot=24), dict(rot=80), dict(n_pos=0), dict(ld=511), dict(ld=514),
+                dict(dtype=L.DT_BF16, ld=516)):
+        assert _append(c, **bad) == L.ERR_ARG, bad
+    assert _append(c, dtype=L.DT_I32) == L.ERR_UNSUPPORTED
+    assert _append(c, T=0) == L.OK
+    assert L.lib().sm100_paged_read(ctypes.byref(c), P, P, P, P + 2, 1, None) == L.ERR_ARG
+    assert L.lib().sm100_paged_read(ctypes.byref(c), P, P, P, P, 0, None) == L.OK
+
+
+def test_attention_refusals():
+    c = _cache()
+    for bad in (dict(q=None), dict(kv_len=None), dict(out=None), dict(ws=None), dict(T=-1), dict(heads=3),
+                dict(max_rows=0), dict(q_off=None, T=1), dict(q_off=None, max_rows=2), dict(q=P + 8), dict(out=P + 8),
+                dict(ws=P + 8), dict(ld_q=100), dict(ld_q=260), dict(ws_bytes=0)):
+        assert _attend(c, **bad) == L.ERR_ARG, bad
+    assert _attend(c, T=0) == L.OK
+    assert L.lib().sm100_paged_attention_ws_bytes(ctypes.byref(c), 4, 1) > 0
+
+
+def test_sample_refusals():
+    for bad in (dict(logits=None), dict(noise=None), dict(tok=None), dict(B=-1), dict(V=0), dict(ld=7), dict(ld_noise=7),
+                dict(ld=-1)):
+        assert _sample(**bad) == L.ERR_ARG, bad
+    assert _sample(dtype=L.DT_I32) == L.ERR_UNSUPPORTED
+    assert _sample(B=0) == L.OK

@@ -107,6 +107,31 @@ class Sm100SkinnyArgs(ctypes.Structure):
         ("flags", c_int32), ("kv_ctx", c_int32), ("ln_g", c_void_p), ("ln_b", c_void_p), ("eps", c_float)]
 
 
+KV_Q4, KV_BF16 = 4, 16
+
+
+class Sm100PagedCache(ctypes.Structure):
+    """include/thvm_sm100.h Sm100PagedCache: a pool of key / value pages and its table."""
+    _fields_ = [("pool", c_void_p), ("table", c_void_p)] + [
+        (n, c_int32) for n in ("n_pages", "page", "kv_heads", "head_dim", "bits", "n_seq", "max_pages")]
+
+
+class Sm100PagedAppendArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("qkv", "g_q", "g_k", "cos_t", "sin_t", "pos", "seq", "q_out")] + [
+        ("ld", c_int64)] + [(n, c_int32) for n in ("T", "heads", "dtype", "rot", "n_pos", "pairs")] + [("eps", c_float)]
+
+
+class Sm100PagedAttnArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("q", "kv_len", "q_off", "out", "ws")] + [
+        ("ws_bytes", c_uint64), ("ld_q", c_int64)] + [(n, c_int32) for n in ("T", "heads", "max_rows")] + [
+        ("scale", c_float)]
+
+
+class Sm100SampleArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("logits", "noise", "temperature", "top_k", "top_p", "min_p", "tok", "logp")] + [
+        ("ld", c_int64), ("ld_noise", c_int64)] + [(n, c_int32) for n in ("B", "V", "dtype")]
+
+
 _PL = ctypes.c_void_p * DECODE_MAX_LAYERS
 
 
@@ -261,6 +286,13 @@ SIGNATURES = {
                                                c_int32, c_int32, c_float, c_void_p]),
     "sm100_comm_pick": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
     "sm100_comm_status": (c_uint32, []),
+    "sm100_paged_block_bytes": (c_uint64, [c_int32, c_int32, c_int32]),
+    "sm100_paged_append": (c_int, [c_void_p, c_void_p, c_void_p]),
+    "sm100_paged_read": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p]),
+    "sm100_paged_attention": (c_int, [c_void_p, c_void_p, c_void_p]),
+    "sm100_paged_attention_ws_bytes": (c_uint64, [c_void_p, c_int32, c_int32]),
+    "sm100_paged_status": (c_uint32, []),
+    "sm100_sample": (c_int, [c_void_p, c_void_p]),
     "sm100_safetensors_load": (c_int, [ctypes.c_char_p, POINTER(Sm100TensorEntry), c_int32, POINTER(c_int32)]),
     "sm100_dsv2pack_load": (c_int, [ctypes.c_char_p, POINTER(Sm100TensorEntry), c_int32, POINTER(c_int32)]),
     "sm100_torch_load": (c_int, [ctypes.c_char_p, POINTER(Sm100TensorEntry), c_int32, POINTER(c_int32)]),

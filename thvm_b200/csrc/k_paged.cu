@@ -1,0 +1,356 @@
+// Writing the paged key / value cache: per-head RMS norm of queries and keys,
+// position rotation, and the append of keys and values in bf16 or 4 bits, in
+// one pass over the rows of a fused projection; and reading it back as values.
+//
+// Per head x[hd] of a row at position p: y = x * rsqrt(sum x^2 / hd + eps) * g
+// (queries and keys, where there is a g); (y_a, y_b) -> (y_a cos - y_b sin,
+// y_b cos + y_a sin) over the rotated pairs; then one rounding: bf16, or per 64
+// dimensions m = bf16(min), s = bf16((max - min) / 15), code = round((y - m) /
+// s) clamped to 0..15.  The codes are taken against the rounded m and s, so
+// their rounding does not add to the value's error except at the ends.
+//
+// A thread holds 8 neighbouring dimensions in f32 (one 16-byte load of bf16,
+// two of f32), a head is hd / 8 neighbouring lanes: the norm's sum, the
+// half-apart rotation partner and the group's extremes are shuffles within
+// them, so nothing passes through shared memory.
+#include "paged.cuh"
+
+using namespace sm100;
+
+namespace {
+
+struct AppendParams {
+  const void *qkv;
+  const float *g_q, *g_k, *cos_t, *sin_t;
+  const int32_t *pos, *seq;
+  __nv_bfloat16 *q_out;
+  int64_t ld, items;   // items: T * (heads + 2 kv_heads)
+  int heads, rot, n_pos, pairs;
+  float eps;
+};
+
+__device__ __forceinline__ void load8(const float *p, float x[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+
+__device__ __forceinline__ void load8(const __nv_bfloat16 *p, float x[8]) {
+  const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[2 * i] = bf16_lo(w[i]), x[2 * i + 1] = bf16_hi(w[i]);
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+__device__ __forceinline__ uint4 pack8(const float x[8]) {
+  return make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+}
+
+// min / max that keep a NaN (a group with one must not read as numbers)
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ float shfl_add(float v, int o) { return __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, o)); }
+
+// sum x^2 of a head in one fixed order that does not depend on how the head is
+// spread over lanes, each step rounded on its own: squares are added up in
+// runs of `unit` neighbours (256 dimensions: the two halves first), then by
+// halves, element i with element i + n / 2.  A key that a plain evaluation of
+// the formula in this order quantises gets the same codes here, ties included.
+template <int HD>
+__device__ __forceinline__ float sum_squares(const float x[8]) {
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) s[i] = __fmul_rn(x[i], x[i]);
+  if constexpr (HD == 64) {   // unit 1: 32, 16 and 8 apart are lanes, 4, 2 and 1 apart within the lane
+    const int hl = threadIdx.x & 7;
+    float a[4], b[2];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {   // each exchange halves what a lane holds
+      const float got = __shfl_xor_sync(0xffffffffu, hl & 4 ? s[i] : s[i + 4], 4);
+      a[i] = __fadd_rn(hl & 4 ? s[i + 4] : s[i], got);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const float got = __shfl_xor_sync(0xffffffffu, hl & 2 ? a[i] : a[i + 2], 2);
+      b[i] = __fadd_rn(hl & 2 ? a[i + 2] : a[i], got);
+    }
+    const float got = __shfl_xor_sync(0xffffffffu, hl & 1 ? b[0] : b[1], 1);
+    const float c = __fadd_rn(hl & 1 ? b[1] : b[0], got);   // dimension hl of each of the 8 runs of 8
+    return shfl_add(shfl_add(shfl_add(c, 4), 2), 1);
+  } else {   // unit 4: two runs a lane
+    if constexpr (HD == 256) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) s[i] = shfl_add(s[i], 16);
+    }
+    float lo = __fadd_rn(__fadd_rn(__fadd_rn(s[0], s[1]), s[2]), s[3]);
+    float hi = __fadd_rn(__fadd_rn(__fadd_rn(s[4], s[5]), s[6]), s[7]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) lo = shfl_add(lo, o), hi = shfl_add(hi, o);
+    return __fadd_rn(lo, hi);
+  }
+}
+
+template <int HD, int BITS, typename In>
+__global__ void __launch_bounds__(256) paged_append_kernel(const PagedView c, const AppendParams a) {
+  constexpr int L = HD / 8;   // lanes of a head
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, hl = lane % L;
+  int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
+  const bool live = item < a.items;
+  if (!live) item = a.items - 1;   // idle lanes follow the last head: the shuffles take whole warps
+  const int n_heads = a.heads + 2 * c.kv_heads;
+  const int64_t t = item / n_heads;
+  const int h = (int)(item - t * n_heads);
+  pdl_wait();
+  float x[8];
+  load8(static_cast<const In *>(a.qkv) + t * a.ld + (int64_t)h * HD + hl * 8, x);
+  const int pos = a.pos[t], seq = a.seq[t];
+  const bool is_q = h < a.heads, turns = h < a.heads + c.kv_heads;
+  uint8_t *blk = paged_block(c, seq, pos);
+  const bool ok = blk != nullptr && (a.rot == 0 || pos < a.n_pos);
+  if (!ok && live && hl == 0) atomicOr(&g_paged_status, SM100_DECODE_ERR_ARG);
+  const float *g = is_q ? a.g_q : a.g_k;
+  const bool normed = turns && g != nullptr;
+  const float ss = sum_squares<HD>(x);
+  if (normed) {
+    const float r = rsqrtf(__fadd_rn(ss * (1.0f / HD), a.eps));
+    float w[8];
+    load8(g + hl * 8, w);
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
+  }
+  if (a.rot) {
+    const int half = a.rot / 2, d0 = hl * 8;
+    const bool in = turns && ok && d0 < a.rot;
+    if (a.pairs) {
+      if (in) {
+        const float4 cs = __ldg(reinterpret_cast<const float4 *>(a.cos_t + (int64_t)pos * half + d0 / 2));
+        const float4 sn = __ldg(reinterpret_cast<const float4 *>(a.sin_t + (int64_t)pos * half + d0 / 2));
+        const float cc[4] = {cs.x, cs.y, cs.z, cs.w}, nn[4] = {sn.x, sn.y, sn.z, sn.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float u = x[2 * i], w = x[2 * i + 1];
+          x[2 * i] = __fsub_rn(__fmul_rn(u, cc[i]), __fmul_rn(w, nn[i]));
+          x[2 * i + 1] = __fadd_rn(__fmul_rn(w, cc[i]), __fmul_rn(u, nn[i]));
+        }
+      }
+    } else {
+      const bool low = d0 < half;
+      const int src = d0 < a.rot ? (low ? lane + half / 8 : lane - half / 8) : lane;
+      float cc[8], nn[8];
+      if (in) {
+        const int64_t at = (int64_t)pos * half + (low ? d0 : d0 - half);
+        load8(a.cos_t + at, cc);
+        load8(a.sin_t + at, nn);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float y = __shfl_sync(0xffffffffu, x[i], src);
+        if (in) {
+          const float u = __fmul_rn(x[i], cc[i]), w = __fmul_rn(y, nn[i]);
+          x[i] = low ? __fsub_rn(u, w) : __fadd_rn(u, w);
+        }
+      }
+    }
+  }
+  if (is_q) {
+    if (live)
+      *reinterpret_cast<uint4 *>(a.q_out + (t * a.heads + h) * HD + hl * 8) = ok ? pack8(x) : make_uint4(0, 0, 0, 0);
+  }
+  const bool is_v = !turns;
+  const int kh = h - a.heads - (is_v ? c.kv_heads : 0);
+  const int row = pos & (c.page - 1);
+  const bool store = live && ok && !is_q;
+  uint8_t *dst = blk + (int64_t)kh * c.block + (is_v ? c.block / 2 : 0);
+  if constexpr (BITS == 16) {
+    if (store) *reinterpret_cast<uint4 *>(dst + ((int64_t)row * HD + hl * 8) * 2) = pack8(x);
+  } else {
+    float mn = x[0], mx = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) mn = min_nan(mn, x[i]), mx = max_nan(mx, x[i]);
+#pragma unroll
+    for (int o = kGroup / 16; o > 0; o >>= 1) {   // the 8 lanes of a group
+      mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+    const __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(__fsub_rn(mx, mn), 1.0f / 15.0f)), mb = __float2bfloat16_rn(mn);
+    const float s = __bfloat162float(sb), m = __bfloat162float(mb);
+    uint32_t codes = 0;
+    if (s > 0.0f) {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        codes |= (uint32_t)fminf(fmaxf(rintf((x[i] - m) / s), 0.0f), 15.0f) << (4 * i);
+    }
+    if (store) {
+      *reinterpret_cast<uint32_t *>(dst + (int64_t)row * (HD / 2) + hl * 4) = codes;
+      if (hl % 8 == 0) {
+        const __nv_bfloat162 pr = __halves2bfloat162(sb, mb);
+        *reinterpret_cast<__nv_bfloat162 *>(dst + (int64_t)c.page * (HD / 2) + ((int64_t)row * (HD / kGroup) + hl / 8) * 4) = pr;
+      }
+    }
+  }
+}
+
+template <int HD, int BITS>
+__global__ void __launch_bounds__(256) paged_read_kernel(const PagedView c, const int32_t *pos, const int32_t *seq,
+                                                         __nv_bfloat16 *k, __nv_bfloat16 *v, int64_t items) {
+  constexpr int L = HD / 8;
+  pdl_trigger();
+  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;   // (t, key head, keys | values)
+  const int hl = threadIdx.x % L;
+  pdl_wait();
+  if (item >= items) return;
+  const int64_t t = item / (2 * c.kv_heads);
+  const int r = (int)(item - t * 2 * c.kv_heads), kh = r >> 1, is_v = r & 1;
+  const int p = pos[t];
+  const uint8_t *blk = paged_block(c, seq[t], p);
+  uint4 out = make_uint4(0, 0, 0, 0);
+  if (!blk) {
+    if (hl == 0) atomicOr(&g_paged_status, SM100_DECODE_ERR_ARG);
+  } else {
+    const uint8_t *src = blk + (int64_t)kh * c.block + (is_v ? c.block / 2 : 0);
+    const int row = p & (c.page - 1);
+    if constexpr (BITS == 16) {
+      out = *reinterpret_cast<const uint4 *>(src + ((int64_t)row * HD + hl * 8) * 2);
+    } else {
+      const uint32_t codes = *reinterpret_cast<const uint32_t *>(src + (int64_t)row * (HD / 2) + hl * 4);
+      const uint32_t sm = *reinterpret_cast<const uint32_t *>(src + (int64_t)c.page * (HD / 2) +
+                                                              ((int64_t)row * (HD / kGroup) + hl / 8) * 4);
+      const float s = bf16_lo(sm), m = bf16_hi(sm);
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = __fadd_rn(m, __fmul_rn((float)((codes >> (4 * i)) & 15u), s));
+      out = pack8(x);
+    }
+  }
+  *reinterpret_cast<uint4 *>((is_v ? v : k) + (t * c.kv_heads + kh) * HD + hl * 8) = out;
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+extern "C" uint64_t sm100_paged_block_bytes(int32_t page, int32_t head_dim, int32_t bits) {
+  if ((page != 16 && page != 32 && page != 64) || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return 0;
+  if (bits == SM100_KV_BF16) return 4ull * page * head_dim;
+  if (bits == SM100_KV_Q4) return 2ull * page * (head_dim / 2 + 4 * (head_dim / kGroup));
+  return 0;
+}
+
+int sm100_paged_view(const Sm100PagedCache *c, const char *what, PagedView *v) {
+  if (!c || !c->pool || !c->table) return sm100_set_error(SM100_ERR_ARG, "%s: no cache", what);
+  const uint64_t block = sm100_paged_block_bytes(c->page, c->head_dim, c->bits);
+  if (!block)
+    return sm100_set_error(SM100_ERR_UNSUPPORTED,
+                           "%s: page %d (16, 32, 64), head_dim %d (64, 128, 256), bits %d (4, 16)", what, c->page,
+                           c->head_dim, c->bits);
+  if (c->n_pages < 1 || c->kv_heads < 1 || c->n_seq < 1 || c->max_pages < 1 ||
+      (int64_t)c->max_pages * c->page > INT32_MAX || !aligned16(c->pool))
+    return sm100_set_error(SM100_ERR_ARG, "%s: n_pages %d kv_heads %d n_seq %d max_pages %d, pool 16-byte aligned",
+                           what, c->n_pages, c->kv_heads, c->n_seq, c->max_pages);
+  v->pool = static_cast<uint8_t *>(c->pool);
+  v->table = c->table;
+  v->n_pages = c->n_pages;
+  v->page = c->page;
+  v->page_log2 = c->page == 16 ? 4 : c->page == 32 ? 5 : 6;
+  v->kv_heads = c->kv_heads;
+  v->n_seq = c->n_seq;
+  v->max_pages = c->max_pages;
+  v->block = (uint32_t)block;
+  return SM100_OK;
+}
+
+namespace {
+
+template <int HD>
+cudaError_t append_hd(const PagedView &v, int bits, int dtype, const AppendParams &p, cudaStream_t st) {
+  const int64_t blocks = (p.items * (HD / 8) + 255) / 256;
+  const dim3 grid((unsigned)blocks), block(256);
+  if (bits == 16)
+    return dtype == SM100_DT_F32 ? launch_pdl(paged_append_kernel<HD, 16, float>, grid, block, 0, st, v, p)
+                                 : launch_pdl(paged_append_kernel<HD, 16, __nv_bfloat16>, grid, block, 0, st, v, p);
+  return dtype == SM100_DT_F32 ? launch_pdl(paged_append_kernel<HD, 4, float>, grid, block, 0, st, v, p)
+                               : launch_pdl(paged_append_kernel<HD, 4, __nv_bfloat16>, grid, block, 0, st, v, p);
+}
+
+}  // namespace
+
+extern "C" int sm100_paged_append(const Sm100PagedCache *c, const Sm100PagedAppendArgs *a, void *stream) {
+  PagedView v;
+  if (int rc = sm100_paged_view(c, "paged_append", &v)) return rc;
+  if (a && a->T == 0) return SM100_OK;
+  if (!a || !a->qkv || !a->pos || !a->seq || !a->q_out || a->T < 0 || a->heads < 1 || a->heads % c->kv_heads)
+    return sm100_set_error(SM100_ERR_ARG, "paged_append: T %d heads %d (a multiple of kv_heads %d)", a ? a->T : 0,
+                           a ? a->heads : 0, c->kv_heads);
+  if (a->dtype != SM100_DT_F32 && a->dtype != SM100_DT_BF16)
+    return sm100_set_error(SM100_ERR_UNSUPPORTED, "paged_append: qkv dtype %d (f32 or bf16)", a->dtype);
+  const int64_t width = ((int64_t)a->heads + 2 * c->kv_heads) * c->head_dim, ld = a->ld ? a->ld : width;
+  const bool rot = a->cos_t || a->sin_t;
+  if (rot && (!a->cos_t || !a->sin_t || a->rot < 16 || a->rot % 16 || a->rot > c->head_dim || a->n_pos < 1 ||
+              !aligned16(a->cos_t) || !aligned16(a->sin_t)))
+    return sm100_set_error(SM100_ERR_ARG, "paged_append: rot %d (a multiple of 16 up to head_dim), n_pos %d, both tables",
+                           a->rot, a->n_pos);
+  if (ld < width || ld % (a->dtype == SM100_DT_F32 ? 4 : 8) || !aligned16(a->qkv) || !aligned16(a->q_out) ||
+      (a->g_q && !aligned16(a->g_q)) || (a->g_k && !aligned16(a->g_k)))
+    return sm100_set_error(SM100_ERR_ARG, "paged_append: row stride %lld of %lld elements, 16-byte rows and addresses",
+                           (long long)ld, (long long)width);
+  AppendParams p{a->qkv, a->g_q, a->g_k, a->cos_t, a->sin_t, a->pos, a->seq, static_cast<__nv_bfloat16 *>(a->q_out),
+                 ld, (int64_t)a->T * (a->heads + 2 * c->kv_heads), a->heads, rot ? a->rot : 0, a->n_pos, a->pairs,
+                 a->eps};
+  if (p.items * (c->head_dim / 8) / 256 >= INT32_MAX)
+    return sm100_set_error(SM100_ERR_ARG, "paged_append: %d rows in one call", a->T);
+  cudaStream_t st = (cudaStream_t)stream;
+  const cudaError_t e = c->head_dim == 64    ? append_hd<64>(v, c->bits, a->dtype, p, st)
+                        : c->head_dim == 128 ? append_hd<128>(v, c->bits, a->dtype, p, st)
+                                             : append_hd<256>(v, c->bits, a->dtype, p, st);
+  if (e != cudaSuccess) return sm100_set_error(SM100_ERR_CUDA, "paged_append: %s", cudaGetErrorString(e));
+  return launch_status("paged_append");
+}
+
+extern "C" int sm100_paged_read(const Sm100PagedCache *c, const int32_t *pos, const int32_t *seq, void *k, void *v,
+                                int32_t T, void *stream) {
+  PagedView w;
+  if (int rc = sm100_paged_view(c, "paged_read", &w)) return rc;
+  if (T == 0) return SM100_OK;
+  if (!pos || !seq || !k || !v || T < 0 || !aligned16(k) || !aligned16(v))
+    return sm100_set_error(SM100_ERR_ARG, "paged_read: T %d, k and v 16-byte aligned", T);
+  const int64_t items = (int64_t)T * 2 * c->kv_heads, blocks = (items * (c->head_dim / 8) + 255) / 256;
+  if (blocks >= INT32_MAX) return sm100_set_error(SM100_ERR_ARG, "paged_read: %d rows in one call", T);
+  const dim3 grid((unsigned)blocks), block(256);
+  auto *ko = static_cast<__nv_bfloat16 *>(k), *vo = static_cast<__nv_bfloat16 *>(v);
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool q4 = c->bits == SM100_KV_Q4;
+  cudaError_t e;
+  if (c->head_dim == 64)
+    e = q4 ? launch_pdl(paged_read_kernel<64, 4>, grid, block, 0, st, w, pos, seq, ko, vo, items)
+           : launch_pdl(paged_read_kernel<64, 16>, grid, block, 0, st, w, pos, seq, ko, vo, items);
+  else if (c->head_dim == 128)
+    e = q4 ? launch_pdl(paged_read_kernel<128, 4>, grid, block, 0, st, w, pos, seq, ko, vo, items)
+           : launch_pdl(paged_read_kernel<128, 16>, grid, block, 0, st, w, pos, seq, ko, vo, items);
+  else
+    e = q4 ? launch_pdl(paged_read_kernel<256, 4>, grid, block, 0, st, w, pos, seq, ko, vo, items)
+           : launch_pdl(paged_read_kernel<256, 16>, grid, block, 0, st, w, pos, seq, ko, vo, items);
+  if (e != cudaSuccess) return sm100_set_error(SM100_ERR_CUDA, "paged_read: %s", cudaGetErrorString(e));
+  return launch_status("paged_read");
+}
+
+extern "C" uint32_t sm100_paged_status(void) {
+  uint32_t v = 0, z = 0;
+  cudaDeviceSynchronize();
+  cudaMemcpyFromSymbol(&v, g_paged_status, sizeof(v));
+  cudaMemcpyToSymbol(g_paged_status, &z, sizeof(z));
+  return v | sm100_paged_attn_take_status();
+}
