@@ -258,7 +258,7 @@ int sm100_paged_view(const Sm100PagedCache *c, const char *what, PagedView *v) {
                            "%s: page %d (16, 32, 64), head_dim %d (64, 128, 256), bits %d (4, 16)", what, c->page,
                            c->head_dim, c->bits);
   if (c->n_pages < 1 || c->kv_heads < 1 || c->n_seq < 1 || c->max_pages < 1 ||
-      (int64_t)c->max_pages * c->page > INT32_MAX || !aligned16(c->pool))
+      (int64_t)c->max_pages * c->page > 1 << 30 || !aligned16(c->pool))
     return sm100_set_error(SM100_ERR_ARG, "%s: n_pages %d kv_heads %d n_seq %d max_pages %d, pool 16-byte aligned",
                            what, c->n_pages, c->kv_heads, c->n_seq, c->max_pages);
   v->pool = static_cast<uint8_t *>(c->pool);
