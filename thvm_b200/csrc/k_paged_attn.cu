@@ -30,9 +30,12 @@
 // queries, and unpacked codes written back to shared memory.)
 //
 // 4 bits: a code c enters the products as an exact bf16 integer (128 + c in
-// K, put together by one AND-OR; c - 8 in V).  A group's scale and minimum
-// are applied outside: S = s * (Q . (128 + c)) + (m - 128 s) * sum Q per group of
-// 64 dimensions, and p * s per token is V's weight, sum p (m + 8 s) its shift.
+// K, 16 + c in V, each put together by a shift and one AND-OR; the offset of V
+// is the smaller one since its sums cancel).  A group's scale and minimum are
+// applied outside: S = s * (Q . (128 + c)) + (m - 128 s) * sum Q per group of 64
+// dimensions, and p * s per token is V's weight, sum p (m - 16 s) its shift.
+// Weights enter as bf16 hi + lo, so their rounding (2^-17) is far below the
+// output's.
 #include "paged.cuh"
 #include "tma.cuh"
 
@@ -55,19 +58,22 @@ constexpr int kMaxPieces = 148 * 4;   // CTAs of a launch at most
 
 template <int HD, int BITS, int NT>
 struct Shape {
-  static constexpr int NW = BITS == 4 ? 8 : 4;                  // warps at the products
-  static constexpr int TS = 16 * NW;                            // tokens of a tile
+  static constexpr int NW = 4;                                  // warps at the products
+  static constexpr int KS = BITS == 4 || HD == 64 ? 2 : 1;      // 16-token steps that a warp takes of a tile
+  static constexpr int TS = 16 * KS * NW;                       // tokens of a tile
   static constexpr int TOKEN = BITS == 4 ? HD / 2 + HD / kGroup * 4 : 2 * HD;
   static constexpr int TILE = 2 * TS * TOKEN;                   // bytes of a tile
   static constexpr int NC = 8 * NT;                             // query columns
-  static constexpr int CTAS = HD == 256 || (BITS == 4 && NT == 2) ? 1 : 2;   // per SM
-  static constexpr int RING = HD == 256 ? 196608 : 98304;       // bytes for stages
-  static constexpr int STAGES = RING / TILE > 8 ? 8 : RING / TILE;
   static constexpr int CHUNK = 16;                              // accumulators joined at a time
   static constexpr int ACC = HD / 16 * NT * 4;                  // accumulators of a thread
   static constexpr int PART = ACC * 32 + 2 * NC;                // floats of a unit's part
   static constexpr int RED = NW * CHUNK * 32 * 4;
-  static constexpr int SMEM = STAGES * TILE + RED + 1024;
+  // CTAs of an SM: what the registers leave (5 warps each: 128 registers at 3, 168 at 2)
+  static constexpr int CTAS = HD == 256 ? (BITS == 4 ? 2 : 1) : NT == 2 || (HD == 128 && BITS == 16) ? 2 : 3;
+  static constexpr int ROOM = 227 * 1024 / CTAS - RED - 3072;
+  static constexpr int STAGES = ROOM / TILE > 8 ? 8 : ROOM / TILE;
+  static constexpr int SMEM = STAGES * TILE + RED;
+  static_assert(STAGES >= 2, "a ring needs two stages");
 };
 
 __device__ __forceinline__ void mma_bf16(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
@@ -103,85 +109,102 @@ __device__ __forceinline__ void split_weights(float w0, float w1, uint32_t &hi, 
 
 // two codes of a word (bits 4 i and 4 i + 16) as bf16 128 + c
 __device__ __forceinline__ uint32_t codes128(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u; }
-// the same as bf16 c - 8
-__device__ __forceinline__ uint32_t codes8(uint32_t w, int i) {
-  const uint32_t v = codes128(w, i);
-  __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162 *>(&v);
-  x = __hsub2(x, __floats2bfloat162_rn(136.0f, 136.0f));
-  return *reinterpret_cast<const uint32_t *>(&x);
+// the same as bf16 16 + c (the code in the upper four bits of the mantissa)
+__device__ __forceinline__ uint32_t codes16(uint32_t w, int i) {
+  return ((i == 0 ? w << 3 : w >> (4 * i - 3)) & 0x00780078u) | 0x41804180u;
 }
 
-// The line of tiles, in the order (sequence, key head, column tile, token tile).
+// The line: units in the order (sequence, key head, column tile), each kPad
+// places for what a unit costs beside its tiles (queries, joining, output:
+// about that many tiles' time), then its token tiles.
+constexpr int kPad = 2;
+
 template <int TS, int NC>
 struct Line {
   const AttnParams *a;
   const PagedView *c;
   int s, h, ct, n_ct, rows, first, len;   // the current unit
-  int tiles, skip;                        // its tiles; how many lie before the piece
+  int tiles;                              // its tiles
+  int64_t at;                             // its first place
 
   __device__ __forceinline__ void load(int seq, int &r, int &f, int &l) const {
     f = a->q_off ? a->q_off[seq] : seq;
     r = a->q_off ? a->q_off[seq + 1] - f : 1;
+    l = a->kv_len[seq];
     if (f < 0 || r < 0 || f > a->T - r) r = 0;   // rows outside q: none
-    l = min(max(a->kv_len[seq], 0), c->max_pages * c->page);
+    l = min(max(l, 0), c->max_pages * c->page);
   }
   __device__ __forceinline__ int columns(int r) const { return (r * a->group + NC - 1) / NC; }
-  // keys that the last row of a column tile sees
-  __device__ __forceinline__ int keys(int r, int l, int t) const {
-    const int last = min(r * a->group, (t + 1) * NC) - 1;
-    return l - r + last / a->group + 1;
-  }
+  // token tiles up to the last key that a column tile's last row sees
   __device__ __forceinline__ int unit_tiles(int r, int l, int t) const {
-    const int k = keys(r, l, t);
+    const int last = min(r * a->group, (t + 1) * NC) - 1;
+    const int k = l - r + last / a->group + 1;
     return k <= TS ? 1 : (k + TS - 1) / TS;   // a unit without keys still has its output to write
   }
-  __device__ __forceinline__ int64_t seq_tiles(int seq) const {
-    int r, f, l;
+  __device__ __forceinline__ int64_t head_places(int r, int l) const {
     int64_t n = 0;
-    load(seq, r, f, l);
-    for (int t = 0, e = columns(r); t < e; t++) n += unit_tiles(r, l, t);
-    return n * c->kv_heads;
-  }
-  __device__ int64_t total(int lane) const {
-    int64_t n = 0;
-    for (int i = lane; i < c->n_seq; i += 32) n += seq_tiles(i);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    for (int t = 0, e = columns(r); t < e; t++) n += kPad + unit_tiles(r, l, t);
     return n;
   }
-  // the unit of tile w of the line (w < total)
-  __device__ void seek(int64_t w, int lane) {
-    int64_t before = 0;
-    int base = 0;
-    for (;; base += 32) {
-      const int64_t n = base + lane < c->n_seq ? seq_tiles(base + lane) : 0;
+  // Cuts the line into pieces for `ctas` CTAs and goes to the first unit of
+  // piece `me`: [w0, w1), false where there are fewer pieces.
+  __device__ bool cut(int ctas, int me, int lane, int64_t &total, int &pieces, int64_t &w0, int64_t &w1) {
+    int r = 0, f = 0, l = 0;
+    if (lane < c->n_seq) load(lane, r, f, l);
+    const int64_t n0 = r ? head_places(r, l) * c->kv_heads : 0;   // sequences 0 .. 31 stay in registers
+    total = n0;
+    for (int i = lane + 32; i < c->n_seq; i += 32) {
+      int r1, f1, l1;
+      load(i, r1, f1, l1);
+      total += head_places(r1, l1) * c->kv_heads;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    pieces = (int)min((int64_t)ctas, total);   // every piece holds a place
+    if (me >= pieces) return false;
+    w0 = total * me / pieces;
+    w1 = total * (me + 1) / pieces;
+    at = 0;
+    int64_t n = n0;
+    for (int base = 0;; base += 32) {
+      if (base) {
+        r = 0;
+        if (base + lane < c->n_seq) load(base + lane, r, f, l);
+        n = r ? head_places(r, l) * c->kv_heads : 0;
+      }
       int64_t up = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t v = __shfl_up_sync(0xffffffffu, up, o);
         if (lane >= o) up += v;
       }
-      const uint32_t past = __ballot_sync(0xffffffffu, before + up > w);
+      const uint32_t past = __ballot_sync(0xffffffffu, at + up > w0);
       if (past) {
-        const int at = __ffs(past) - 1;
-        s = base + at;
-        before += __shfl_sync(0xffffffffu, up - n, at);
+        const int hit = __ffs(past) - 1;
+        s = base + hit;
+        at += __shfl_sync(0xffffffffu, up - n, hit);
+        rows = __shfl_sync(0xffffffffu, r, hit);
+        first = __shfl_sync(0xffffffffu, f, hit);
+        len = __shfl_sync(0xffffffffu, l, hit);
         break;
       }
-      before += __shfl_sync(0xffffffffu, up, 31);
+      at += __shfl_sync(0xffffffffu, up, 31);
     }
-    load(s, rows, first, len);
     n_ct = columns(rows);
-    int64_t left = w - before, per = 0;
-    for (int t = 0; t < n_ct; t++) per += unit_tiles(rows, len, t);
-    h = (int)(left / per);
-    left -= h * per;
+    const int64_t per = head_places(rows, len);
+    h = (int)((w0 - at) / per);
+    at += h * per;
     ct = 0;
-    while (left >= (tiles = unit_tiles(rows, len, ct))) left -= tiles, ct++;
-    skip = (int)left;
+    for (;;) {
+      tiles = unit_tiles(rows, len, ct);
+      if (w0 < at + kPad + tiles) break;
+      at += kPad + tiles;
+      ct++;
+    }
+    return true;
   }
   __device__ __forceinline__ void next() {
-    skip = 0;
+    at += kPad + tiles;
     if (++ct == n_ct) {
       ct = 0;
       if (++h == c->kv_heads) {
@@ -193,17 +216,22 @@ struct Line {
     }
     tiles = unit_tiles(rows, len, ct);
   }
+  // the piece's tiles of the current unit: [t0, t1), empty where it ends inside the unit's first places
+  __device__ __forceinline__ void span(int64_t w0, int64_t w1, int &t0, int &t1) const {
+    t0 = (int)max(w0 - at - kPad, (int64_t)0);
+    t1 = (int)min(w1 - at - kPad, (int64_t)tiles);
+  }
 };
 
 template <int HD, int BITS, int NT>
 __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, BITS, NT>::CTAS)
     paged_attn_kernel(const __grid_constant__ PagedView c, const __grid_constant__ AttnParams a) {
   using S = Shape<HD, BITS, NT>;
-  constexpr int NW = S::NW, TS = S::TS, NC = S::NC, STAGES = S::STAGES, GR = HD / kGroup;
+  constexpr int NW = S::NW, KS = S::KS, TS = S::TS, NC = S::NC, STAGES = S::STAGES, GR = HD / kGroup;
   extern __shared__ __align__(128) uint8_t smem[];
   float *red = reinterpret_cast<float *>(smem + STAGES * S::TILE);
   __shared__ uint64_t full[STAGES], empty[STAGES];
-  __shared__ uint16_t valid[STAGES][NW];
+  __shared__ uint16_t valid[STAGES][TS / 16];
   __shared__ float wm[NW][NC], wl[NW][NC], um[NC], ul[NC];
   __shared__ uint32_t arrived;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -220,12 +248,10 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
   Line<TS, NC> line;
   line.a = &a;
   line.c = &c;
-  const int64_t total = line.total(lane);
-  const int G = (int)min((int64_t)gridDim.x, total), me = blockIdx.x;   // every piece holds a tile
-  if (me >= G) return;
-  const int64_t w0 = total * me / G, w1 = total * (me + 1) / G;
-  line.seek(w0, lane);
-  int64_t w = w0;
+  const int me = blockIdx.x;
+  int64_t total, w0, w1;
+  int G, t0, t1;
+  if (!line.cut(gridDim.x, me, lane, total, G, w0, w1)) return;
   uint32_t it = 0;   // tiles through the ring
 
   if (warp == NW) {
@@ -234,9 +260,9 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
     const uint32_t block = c.block;
     const uint64_t pol = policy_evict_first();
     bool ok_ring = true;
-    while (w < w1 && ok_ring) {
-      const int end = (int)min((int64_t)line.tiles, line.skip + (w1 - w));
-      for (int t = line.skip; t < end; t++, it++) {
+    for (;;) {
+      line.span(w0, w1, t0, t1);
+      for (int t = t0; t < t1 && ok_ring; t++, it++) {
         const int st = it % STAGES;
         const int slot = t * per + lane, key = slot << c.page_log2;
         int id = -1;
@@ -249,7 +275,7 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
           ok_ring = false;
           break;
         }
-        if (lane < NW) {
+        if (lane < TS / 16) {
           const int base = t * TS + 16 * lane, n = min(max(line.len - base, 0), 16);
           valid[st][lane] = oks >> ((16 * lane) >> c.page_log2) & 1 ? (uint16_t)((1u << n) - 1) : 0;
         }
@@ -260,8 +286,8 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
           bulk_g2s_hint(smem + st * S::TILE + lane * block,
                         c.pool + ((int64_t)id * c.kv_heads + line.h) * block, block, &full[st], pol);
       }
-      w += end - line.skip;
-      if (w < w1) line.next();
+      if (!ok_ring || line.at + kPad + line.tiles >= w1) break;
+      line.next();
     }
     if (lane == 0 && me == 0) {   // lengths past the table were cut
       for (int s = 0; s < c.n_seq; s++)
@@ -273,8 +299,9 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
   // ---- the products
   const int g = lane >> 2, cq = lane & 3;
   bool stalled = false;
-  while (w < w1) {
-    const int end = (int)min((int64_t)line.tiles, line.skip + (w1 - w));
+  for (;; line.next()) {
+    line.span(w0, w1, t0, t1);
+    if (t0 >= t1) break;   // the piece ends before the unit's first tile
     const int n_cols = min(NC, line.rows * a.group - line.ct * NC);
     // Q^T fragments: column g of each 8, this lane's dimensions
     uint32_t qf[NT][HD / 8];
@@ -341,99 +368,113 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
         for (int gr = 0; gr < GR; gr++) z[gr][nt][e] = 0.0f;
       }
 
-    for (int t = line.skip; t < end; t++, it++) {
+    for (int t = t0; t < t1; t++, it++) {
       const int st = it % STAGES;
       if (!stalled) stalled = !mbar_wait(&full[st], (it / STAGES) & 1, &g_paged_status, false);
-      const uint32_t bits = stalled ? 0 : valid[st][warp];
-      const int key0 = t * TS + 16 * warp;
-      if (bits != 0) {
-        // this warp's tokens inside their page block
-        const int page_in = (16 * warp) >> c.page_log2, row_in = (16 * warp) & (c.page - 1);
-        const uint8_t *kb = smem + st * S::TILE + page_in * c.block, *vb = kb + c.block / 2;
-        const bool edge = bits != 0xffffu || key0 + 16 > lim_min;
-        float sc[NT][4];
-        if constexpr (BITS == 4) {
-          const uint8_t *km = kb + c.page * (HD / 2) + (row_in + g) * (GR * 4);
-          kb += (row_in + g) * (HD / 2) + cq * 8;
+      uint32_t bits[KS];
+      uint32_t any_bits = 0;
+#pragma unroll
+      for (int x = 0; x < KS; x++) any_bits |= bits[x] = stalled ? 0 : valid[st][KS * warp + x];
+      if (any_bits != 0) {
+        // this warp's tokens: KS steps of 16, each inside a page's block
+        const uint8_t *kb[KS];
+        int row_in[KS], key0[KS];
+        float sc[KS][NT][4];
+        bool edge[KS];
+#pragma unroll
+        for (int x = 0; x < KS; x++) {
+          const int at = 16 * (KS * warp + x);
+          kb[x] = smem + st * S::TILE + (at >> c.page_log2) * c.block;
+          row_in[x] = at & (c.page - 1);
+          key0[x] = t * TS + at;
+          edge[x] = bits[x] != 0xffffu || key0[x] + 16 > lim_min;
 #pragma unroll
           for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) sc[nt][e] = 0.0f;
+            for (int e = 0; e < 4; e++) sc[x][nt][e] = 0.0f;
+        }
+        if constexpr (BITS == 4) {
 #pragma unroll
-          for (int gr = 0; gr < GR; gr++) {
-            const uint2 w0 = *reinterpret_cast<const uint2 *>(kb + gr * 32);
-            const uint2 w8 = *reinterpret_cast<const uint2 *>(kb + gr * 32 + 8 * (HD / 2));
-            const uint32_t m0 = *reinterpret_cast<const uint32_t *>(km + gr * 4);
-            const uint32_t m8 = *reinterpret_cast<const uint32_t *>(km + gr * 4 + 8 * (GR * 4));
-            float acc[NT][4];
+          for (int gr = 0; gr < GR; gr++)
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+            for (int x = 0; x < KS; x++) {
+              const uint8_t *km = kb[x] + c.page * (HD / 2) + (row_in[x] + g) * (GR * 4) + gr * 4;
+              const uint8_t *kc = kb[x] + (row_in[x] + g) * (HD / 2) + cq * 8 + gr * 32;
+              const uint2 u0 = *reinterpret_cast<const uint2 *>(kc);
+              const uint2 u8 = *reinterpret_cast<const uint2 *>(kc + 8 * (HD / 2));
+              const uint32_t m0 = *reinterpret_cast<const uint32_t *>(km);
+              const uint32_t m8 = *reinterpret_cast<const uint32_t *>(km + 8 * (GR * 4));
+              float acc[NT][4];
 #pragma unroll
-              for (int e = 0; e < 4; e++) acc[nt][e] = 0.0f;
+              for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const uint32_t x0 = i < 2 ? w0.x : w0.y, x8 = i < 2 ? w8.x : w8.y;
-              const int j = 2 * (i & 1);
-              const uint32_t af[4] = {codes128(x0, j), codes128(x8, j), codes128(x0, j + 1), codes128(x8, j + 1)};
+                for (int e = 0; e < 4; e++) acc[nt][e] = 0.0f;
 #pragma unroll
-              for (int nt = 0; nt < NT; nt++) mma_bf16(acc[nt], af, qf[nt][8 * gr + 2 * i], qf[nt][8 * gr + 2 * i + 1]);
+              for (int i = 0; i < 4; i++) {
+                const uint32_t x0 = i < 2 ? u0.x : u0.y, x8 = i < 2 ? u8.x : u8.y;
+                const int j = 2 * (i & 1);
+                const uint32_t af[4] = {codes128(x0, j), codes128(x8, j), codes128(x0, j + 1), codes128(x8, j + 1)};
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) mma_bf16(acc[nt], af, qf[nt][8 * gr + 2 * i], qf[nt][8 * gr + 2 * i + 1]);
+              }
+              const float s0 = bf16_lo(m0), s8 = bf16_lo(m8);
+              const float b0 = fmaf(-128.0f, s0, bf16_hi(m0)), b8 = fmaf(-128.0f, s8, bf16_hi(m8));
+#pragma unroll
+              for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                  sc[x][nt][e] = fmaf(s0, acc[nt][e], fmaf(b0, qs[gr][nt][e], sc[x][nt][e]));
+                  sc[x][nt][2 + e] = fmaf(s8, acc[nt][2 + e], fmaf(b8, qs[gr][nt][e], sc[x][nt][2 + e]));
+                }
             }
-            const float s0 = bf16_lo(m0), s8 = bf16_lo(m8);
-            const float b0 = fmaf(-128.0f, s0, bf16_hi(m0)), b8 = fmaf(-128.0f, s8, bf16_hi(m8));
+        } else {
+#pragma unroll
+          for (int i = 0; i < HD / 32; i++)
+#pragma unroll
+            for (int x = 0; x < KS; x++) {
+              const uint8_t *kc = kb[x] + (row_in[x] + g) * (2 * HD) + cq * 16 + i * 64;
+              const uint4 x0 = *reinterpret_cast<const uint4 *>(kc);
+              const uint4 x8 = *reinterpret_cast<const uint4 *>(kc + 8 * (2 * HD));
+              const uint32_t a0[4] = {x0.x, x8.x, x0.y, x8.y}, a1[4] = {x0.z, x8.z, x0.w, x8.w};
+#pragma unroll
+              for (int nt = 0; nt < NT; nt++) {
+                mma_bf16(sc[x][nt], a0, qf[nt][4 * i], qf[nt][4 * i + 1]);
+                mma_bf16(sc[x][nt], a1, qf[nt][4 * i + 2], qf[nt][4 * i + 3]);
+              }
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < KS; x++)
+          if (edge[x]) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-              for (int e = 0; e < 2; e++) {
-                sc[nt][e] = fmaf(s0, acc[nt][e], fmaf(b0, qs[gr][nt][e], sc[nt][e]));
-                sc[nt][2 + e] = fmaf(s8, acc[nt][2 + e], fmaf(b8, qs[gr][nt][e], sc[nt][2 + e]));
+              for (int e = 0; e < 4; e++) {
+                const int r = e < 2 ? g : g + 8;
+                if (!(bits[x] >> r & 1) || key0[x] + r >= lim[nt][e & 1]) sc[x][nt][e] = -INFINITY;
               }
           }
-        } else {
-          kb += (row_in + g) * (2 * HD) + cq * 16;
-#pragma unroll
-          for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) sc[nt][e] = 0.0f;
-#pragma unroll
-          for (int i = 0; i < HD / 32; i++) {
-            const uint4 x0 = *reinterpret_cast<const uint4 *>(kb + i * 64);
-            const uint4 x8 = *reinterpret_cast<const uint4 *>(kb + i * 64 + 8 * (2 * HD));
-            const uint32_t a0[4] = {x0.x, x8.x, x0.y, x8.y}, a1[4] = {x0.z, x8.z, x0.w, x8.w};
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-              mma_bf16(sc[nt], a0, qf[nt][4 * i], qf[nt][4 * i + 1]);
-              mma_bf16(sc[nt], a1, qf[nt][4 * i + 2], qf[nt][4 * i + 3]);
-            }
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) sc[nt][e] *= a.scale_log2;
-        if (edge) {
-#pragma unroll
-          for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const int r = e < 2 ? g : g + 8;
-              if (!(bits >> r & 1) || key0 + r >= lim[nt][e & 1]) sc[nt][e] = -INFINITY;
-            }
-        }
         // the running maximum moves only where a column grows past it by 2^8 (a weight of up to 2^8 costs an f32 sum
         // nothing): most tiles then skip the reduction and the rescaling
+        float top[NT][2];
         bool grows = false;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-          for (int e = 0; e < 2; e++) grows |= fmaxf(sc[nt][e], sc[nt][2 + e]) > m[nt][e] + 8.0f;
+          for (int e = 0; e < 2; e++) {
+            top[nt][e] = fmaxf(sc[0][nt][e], sc[0][nt][2 + e]);
+#pragma unroll
+            for (int x = 1; x < KS; x++) top[nt][e] = fmaxf(top[nt][e], fmaxf(sc[x][nt][e], sc[x][nt][2 + e]));
+            grows |= top[nt][e] * a.scale_log2 > m[nt][e] + 8.0f;
+          }
         if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
           for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              float v = fmaxf(fmaxf(sc[nt][e], sc[nt][2 + e]), m[nt][e]);
+              float v = fmaxf(top[nt][e] * a.scale_log2, m[nt][e]);
 #pragma unroll
-              for (int x = 4; x < 32; x <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
+              for (int y = 4; y < 32; y <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, y));
               const float f = v == -INFINITY ? 1.0f : ex2(m[nt][e] - v);
               m[nt][e] = v;
               l[nt][e] *= f;
@@ -448,103 +489,113 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             const float mm = m[nt][e] == -INFINITY ? 0.0f : m[nt][e];
-            sc[nt][e] = ex2(sc[nt][e] - mm);
-            sc[nt][2 + e] = ex2(sc[nt][2 + e] - mm);
-            l[nt][e] += sc[nt][e] + sc[nt][2 + e];
+#pragma unroll
+            for (int x = 0; x < KS; x++) {
+              sc[x][nt][e] = ex2(fmaf(sc[x][nt][e], a.scale_log2, -mm));
+              sc[x][nt][2 + e] = ex2(fmaf(sc[x][nt][2 + e], a.scale_log2, -mm));
+              l[nt][e] += sc[x][nt][e] + sc[x][nt][2 + e];
+            }
           }
         const int k0 = 2 * cq;   // this lane's tokens of V^T: k0, k0 + 1, k0 + 8, k0 + 9
         if constexpr (BITS == 4) {
-          const uint8_t *vm = vb + c.page * (HD / 2) + (row_in + g) * (GR * 4);
-          vb += (row_in + k0) * (HD / 2) + g * 4;
 #pragma unroll
-          for (int gr = 0; gr < GR; gr++) {
-            const uint32_t m0 = *reinterpret_cast<const uint32_t *>(vm + gr * 4);
-            const uint32_t m8 = *reinterpret_cast<const uint32_t *>(vm + gr * 4 + 8 * (GR * 4));
-            float s0 = bf16_lo(m0), s8 = bf16_lo(m8);
-            float b0 = fmaf(8.0f, s0, bf16_hi(m0)), b8 = fmaf(8.0f, s8, bf16_hi(m8));
-            uint32_t p0[NT], p8[NT], r0[NT], r8[NT];
+          for (int gr = 0; gr < GR; gr++)
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-              float w[4];
-#pragma unroll
-              for (int e = 0; e < 2; e++) {
-                w[e] = sc[nt][e] * s0, w[2 + e] = sc[nt][2 + e] * s8;
-                float d0 = sc[nt][e] * b0, d8 = sc[nt][2 + e] * b8;
-                if (edge) {   // a weight of zero leaves out whatever the token holds
-                  if (sc[nt][e] == 0.0f) w[e] = d0 = 0.0f;
-                  if (sc[nt][2 + e] == 0.0f) w[2 + e] = d8 = 0.0f;
-                }
-                z[gr][nt][e] += d0 + d8;
-              }
-              split_weights(w[0], w[1], p0[nt], r0[nt]);
-              split_weights(w[2], w[3], p8[nt], r8[nt]);
-            }
-            const uint32_t wa = *reinterpret_cast<const uint32_t *>(vb + gr * 32);
-            const uint32_t wb = *reinterpret_cast<const uint32_t *>(vb + gr * 32 + (HD / 2));
-            const uint32_t wc = *reinterpret_cast<const uint32_t *>(vb + gr * 32 + 8 * (HD / 2));
-            const uint32_t wd = *reinterpret_cast<const uint32_t *>(vb + gr * 32 + 9 * (HD / 2));
-            const uint32_t lo[2] = {__byte_perm(wa, wb, 0x5410), __byte_perm(wa, wb, 0x7632)};
-            const uint32_t hi[2] = {__byte_perm(wc, wd, 0x5410), __byte_perm(wc, wd, 0x7632)};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {   // dimensions 8 g + 2 j, 8 g + 2 j + 1 of the group
-              const int i = 2 * (j & 1);
-              const uint32_t af[4] = {codes8(lo[j >> 1], i), codes8(lo[j >> 1], i + 1), codes8(hi[j >> 1], i),
-                                      codes8(hi[j >> 1], i + 1)};
+            for (int x = 0; x < KS; x++) {
+              const uint8_t *vb = kb[x] + c.block / 2;
+              const uint8_t *vm = vb + c.page * (HD / 2) + (row_in[x] + g) * (GR * 4) + gr * 4;
+              vb += (row_in[x] + k0) * (HD / 2) + g * 4 + gr * 32;
+              const uint32_t m0 = *reinterpret_cast<const uint32_t *>(vm);
+              const uint32_t m8 = *reinterpret_cast<const uint32_t *>(vm + 8 * (GR * 4));
+              const uint32_t wa = *reinterpret_cast<const uint32_t *>(vb);
+              const uint32_t wb = *reinterpret_cast<const uint32_t *>(vb + (HD / 2));
+              const uint32_t wc = *reinterpret_cast<const uint32_t *>(vb + 8 * (HD / 2));
+              const uint32_t wd = *reinterpret_cast<const uint32_t *>(vb + 9 * (HD / 2));
+              const float s0 = bf16_lo(m0), s8 = bf16_lo(m8);
+              const float b0 = fmaf(-16.0f, s0, bf16_hi(m0)), b8 = fmaf(-16.0f, s8, bf16_hi(m8));
+              uint32_t p0[NT], p8[NT], r0[NT], r8[NT];
 #pragma unroll
               for (int nt = 0; nt < NT; nt++) {
-                mma_bf16(o[4 * gr + j][nt], af, p0[nt], p8[nt]);
-                mma_bf16(o[4 * gr + j][nt], af, r0[nt], r8[nt]);
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                  w[e] = sc[x][nt][e] * s0, w[2 + e] = sc[x][nt][2 + e] * s8;
+                  float d0 = sc[x][nt][e] * b0, d8 = sc[x][nt][2 + e] * b8;
+                  if (edge[x]) {   // a weight of zero leaves out whatever the token holds
+                    if (sc[x][nt][e] == 0.0f) w[e] = d0 = 0.0f;
+                    if (sc[x][nt][2 + e] == 0.0f) w[2 + e] = d8 = 0.0f;
+                  }
+                  z[gr][nt][e] += d0 + d8;
+                }
+                split_weights(w[0], w[1], p0[nt], r0[nt]);
+                split_weights(w[2], w[3], p8[nt], r8[nt]);
               }
-            }
-          }
-        } else {
-          uint32_t p0[NT], p8[NT], r0[NT], r8[NT];
+              const uint32_t lo[2] = {__byte_perm(wa, wb, 0x5410), __byte_perm(wa, wb, 0x7632)};
+              const uint32_t hi[2] = {__byte_perm(wc, wd, 0x5410), __byte_perm(wc, wd, 0x7632)};
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) {
-            split_weights(sc[nt][0], sc[nt][1], p0[nt], r0[nt]);
-            split_weights(sc[nt][2], sc[nt][3], p8[nt], r8[nt]);
-          }
-          vb += (row_in + k0) * (2 * HD) + g * 16;
-          const int tk[4] = {k0, k0 + 1, k0 + 8, k0 + 9};
-#pragma unroll
-          for (int gr = 0; gr < GR; gr++) {
-            uint4 x[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) x[k] = *reinterpret_cast<const uint4 *>(vb + gr * 128 + (tk[k] - k0) * (2 * HD));
-            if (!edge) {
-#pragma unroll
-              for (int j = 0; j < 4; j++) {
-                const uint32_t wa = (&x[0].x)[j], wb = (&x[1].x)[j], wc = (&x[2].x)[j], wd = (&x[3].x)[j];
-                const uint32_t af[4] = {__byte_perm(wa, wb, 0x5410), __byte_perm(wa, wb, 0x7632),
-                                        __byte_perm(wc, wd, 0x5410), __byte_perm(wc, wd, 0x7632)};
+              for (int j = 0; j < 4; j++) {   // dimensions 8 g + 2 j, 8 g + 2 j + 1 of the group
+                const int i = 2 * (j & 1);
+                const uint32_t af[4] = {codes16(lo[j >> 1], i), codes16(lo[j >> 1], i + 1), codes16(hi[j >> 1], i),
+                                        codes16(hi[j >> 1], i + 1)};
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                   mma_bf16(o[4 * gr + j][nt], af, p0[nt], p8[nt]);
                   mma_bf16(o[4 * gr + j][nt], af, r0[nt], r8[nt]);
                 }
               }
-            } else {
-              // row by row: a token that a row does not see is zeros to it, and another row's product, where that
-              // token may hold an infinity or a NaN, does not enter its columns
-              for (int r = row0; r <= row1; r++) {
-                const int seen = line.len - line.rows + r + 1;
-                uint32_t keep[4];
+            }
+        } else {
+          const int tk[4] = {k0, k0 + 1, k0 + 8, k0 + 9};
 #pragma unroll
-                for (int k = 0; k < 4; k++) keep[k] = (bits >> tk[k] & 1) && key0 + tk[k] < seen ? 0xffffffffu : 0u;
+          for (int x = 0; x < KS; x++) {
+            const uint8_t *vb = kb[x] + c.block / 2 + (row_in[x] + k0) * (2 * HD) + g * 16;
+            uint32_t p0[NT], p8[NT], r0[NT], r8[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+              split_weights(sc[x][nt][0], sc[x][nt][1], p0[nt], r0[nt]);
+              split_weights(sc[x][nt][2], sc[x][nt][3], p8[nt], r8[nt]);
+            }
+#pragma unroll
+            for (int gr = 0; gr < GR; gr++) {
+              uint4 v[4];
+#pragma unroll
+              for (int k = 0; k < 4; k++) v[k] = *reinterpret_cast<const uint4 *>(vb + gr * 128 + (tk[k] - k0) * (2 * HD));
+              if (!edge[x]) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                  const uint32_t wa = (&x[0].x)[j] & keep[0], wb = (&x[1].x)[j] & keep[1];
-                  const uint32_t wc = (&x[2].x)[j] & keep[2], wd = (&x[3].x)[j] & keep[3];
+                  const uint32_t wa = (&v[0].x)[j], wb = (&v[1].x)[j], wc = (&v[2].x)[j], wd = (&v[3].x)[j];
                   const uint32_t af[4] = {__byte_perm(wa, wb, 0x5410), __byte_perm(wa, wb, 0x7632),
                                           __byte_perm(wc, wd, 0x5410), __byte_perm(wc, wd, 0x7632)};
 #pragma unroll
                   for (int nt = 0; nt < NT; nt++) {
-                    float tmp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma_bf16(tmp, af, p0[nt], p8[nt]);
-                    mma_bf16(tmp, af, r0[nt], r8[nt]);
+                    mma_bf16(o[4 * gr + j][nt], af, p0[nt], p8[nt]);
+                    mma_bf16(o[4 * gr + j][nt], af, r0[nt], r8[nt]);
+                  }
+                }
+              } else {
+                // row by row: a token that a row does not see is zeros to it, and another row's product, where that
+                // token may hold an infinity or a NaN, does not enter its columns
+                for (int r = row0; r <= row1; r++) {
+                  const int seen = line.len - line.rows + r + 1;
+                  uint32_t keep[4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                      if (lim[nt][e & 1] == seen) o[4 * gr + j][nt][e] += tmp[e];
+                  for (int k = 0; k < 4; k++)
+                    keep[k] = (bits[x] >> tk[k] & 1) && key0[x] + tk[k] < seen ? 0xffffffffu : 0u;
+#pragma unroll
+                  for (int j = 0; j < 4; j++) {
+                    const uint32_t wa = (&v[0].x)[j] & keep[0], wb = (&v[1].x)[j] & keep[1];
+                    const uint32_t wc = (&v[2].x)[j] & keep[2], wd = (&v[3].x)[j] & keep[3];
+                    const uint32_t af[4] = {__byte_perm(wa, wb, 0x5410), __byte_perm(wa, wb, 0x7632),
+                                            __byte_perm(wc, wd, 0x5410), __byte_perm(wc, wd, 0x7632)};
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                      float tmp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                      mma_bf16(tmp, af, p0[nt], p8[nt]);
+                      mma_bf16(tmp, af, r0[nt], r8[nt]);
+#pragma unroll
+                      for (int e = 0; e < 4; e++)
+                        if (lim[nt][e & 1] == seen) o[4 * gr + j][nt][e] += tmp[e];
+                    }
                   }
                 }
               }
@@ -588,8 +639,8 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
         if (warp == 0 && g == 0) um[col] = top, ul[col] = sum;
       }
     // where the piece ends inside the unit, or began inside it: a part
-    const bool whole = line.skip == 0 && end == line.tiles;
-    float *part = a.parts + ((int64_t)me * 2 + (line.skip == 0)) * S::PART;
+    const bool whole = t0 == 0 && t1 == line.tiles;
+    float *part = a.parts + ((int64_t)me * 2 + (t0 == 0)) * S::PART;
       const auto put = [&](int i, int nt, int e, float v0, float v1) {   // dimensions d, d + 1 of a column
       const int col = nt * 8 + 2 * cq + e, at = line.ct * NC + col;
       if (col >= n_cols) return;
@@ -641,8 +692,8 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
         __stcg(part + S::ACC * 32 + tid, um[tid]);
         __stcg(part + S::ACC * 32 + NC + tid, ul[tid]);
       }
-      // the CTAs that share the unit, by the line's positions of its first and last tile
-      const int64_t u0 = w - line.skip, u1 = u0 + line.tiles - 1;
+      // the CTAs that share the unit, by the places of its first and last tile
+      const int64_t u0 = line.at + kPad, u1 = u0 + line.tiles - 1;
       const int c0 = (int)(((u0 + 1) * G - 1) / total), c1 = (int)(((u1 + 1) * G - 1) / total);
       __threadfence();
       sync();
@@ -651,40 +702,58 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
       if (arrived == (uint32_t)(c1 - c0)) {
         __threadfence();
         if (tid == 0) a.counters[c0] = 0;
-        const float *base = a.parts;
-        const auto part_of = [&](int x) { return base + ((int64_t)x * 2 + (x == c0)) * S::PART; };
-        if (tid < NC) {
+        const auto part_of = [&](int x) { return a.parts + ((int64_t)x * 2 + (x == c0)) * S::PART; };
+        // a column's maximum and sum over the parts, a warp to a column; its weights for kBatch parts at a time
+        constexpr int kBatch = S::RED / 4 / NC;
+        for (int col = warp; col < NC; col += NW) {
           float top = -INFINITY, sum = 0.0f;
-          for (int x = c0; x <= c1; x++) {
-            const float pm = __ldcg(part_of(x) + S::ACC * 32 + tid), pl = __ldcg(part_of(x) + S::ACC * 32 + NC + tid);
+          for (int x = c0 + lane; x <= c1; x += 32) {
+            const float *p = part_of(x) + S::ACC * 32 + col;
+            const float pm = __ldcg(p), pl = __ldcg(p + NC);
             if (pm == -INFINITY) continue;
-            const float t = fmaxf(top, pm);
-            sum = sum * ex2(top - t) + pl * ex2(pm - t);
-            top = t;
+            const float v = fmaxf(top, pm);
+            sum = sum * ex2(top - v) + pl * ex2(pm - v);
+            top = v;
           }
-          um[tid] = top, ul[tid] = sum;
+          const float all = warp_max(top);
+          sum = warp_sum(top == -INFINITY ? 0.0f : sum * ex2(top - all));
+          if (lane == 0) um[col] = all, ul[col] = sum;
         }
-        sync();
-        for (int pr = warp; pr < S::ACC / 2; pr += NW) {
-          const int e = pr & 1, nt = (pr >> 1) % NT, i = (pr >> 1) / NT;
-          const int col = nt * 8 + 2 * cq + e;
-          const float top = um[col];
-          float v0 = 0.0f, v1 = 0.0f;
-#pragma unroll 4
-          for (int x = c0; x <= c1; x++) {
-            const float *p = part_of(x);
-            const float pm = __ldcg(p + S::ACC * 32 + col);
-            const float2 v = __ldcg(reinterpret_cast<const float2 *>(p + pr * 64 + lane * 2));
-            const float fx = pm == -INFINITY ? 0.0f : ex2(pm - top);
-            if (fx != 0.0f) v0 += v.x * fx, v1 += v.y * fx;
+        constexpr int PP = (S::ACC / 2 + NW - 1) / NW;   // pairs of accumulators of a warp
+        float2 v[PP];
+#pragma unroll
+        for (int y = 0; y < PP; y++) v[y] = make_float2(0.0f, 0.0f);
+        for (int x0 = c0; x0 <= c1; x0 += kBatch) {
+          const int n = min(kBatch, c1 - x0 + 1);
+          sync();
+          for (int i = tid; i < n * NC; i += NW * 32) {
+            const float pm = __ldcg(part_of(x0 + i / NC) + S::ACC * 32 + i % NC);
+            red[i] = pm == -INFINITY ? 0.0f : ex2(pm - um[i % NC]);
           }
-          put(i, nt, e, v0, v1);
+          sync();
+#pragma unroll 4
+          for (int x = 0; x < n; x++) {
+            const float *p = part_of(x0 + x) + lane * 2;
+#pragma unroll
+            for (int y = 0; y < PP; y++) {
+              const int pr = y * NW + warp, col = (pr >> 1) % NT * 8 + 2 * cq + (pr & 1);
+              if (pr < S::ACC / 2) {
+                const float2 u = __ldcg(reinterpret_cast<const float2 *>(p + pr * 64));
+                const float f = red[x * NC + col];
+                if (f != 0.0f) v[y].x += u.x * f, v[y].y += u.y * f;
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int y = 0; y < PP; y++) {
+          const int pr = y * NW + warp;
+          if (pr < S::ACC / 2) put((pr >> 1) / NT, (pr >> 1) % NT, pr & 1, v[y].x, v[y].y);
         }
       }
       sync();
     }
-    w += end - line.skip;
-    if (w < w1) line.next();
+    if (line.at + kPad + line.tiles >= w1) break;
   }
   if (stalled && warp == 0)   // a wait gave up: the copies still under way may not outlive the CTA's shared memory
     for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; i++)
