@@ -107,11 +107,18 @@ __device__ __forceinline__ void split_weights(float w0, float w1, uint32_t &hi, 
   lo = transpose8x8(pack2(w0 - bf16_lo(h), w1 - bf16_hi(h)));
 }
 
+// (x & mask) | bits as the one instruction that it is (written plainly it became two, a third of a step's instructions)
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
+  return r;
+}
+
 // two codes of a word (bits 4 i and 4 i + 16) as bf16 128 + c
-__device__ __forceinline__ uint32_t codes128(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u; }
+__device__ __forceinline__ uint32_t codes128(uint32_t w, int i) { return and_or(w >> (4 * i), 0x000f000fu, 0x43004300u); }
 // the same as bf16 16 + c (the code in the upper four bits of the mantissa)
 __device__ __forceinline__ uint32_t codes16(uint32_t w, int i) {
-  return ((i == 0 ? w << 3 : w >> (4 * i - 3)) & 0x00780078u) | 0x41804180u;
+  return and_or(i == 0 ? w << 3 : w >> (4 * i - 3), 0x00780078u, 0x41804180u);
 }
 
 // The line: units in the order (sequence, key head, column tile), each kPad
