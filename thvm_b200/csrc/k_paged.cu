@@ -12,20 +12,29 @@
 // A thread holds 8 neighbouring dimensions in f32 (one 16-byte load of bf16,
 // two of f32), a head is hd / 8 neighbouring lanes: the norm's sum, the
 // half-apart rotation partner and the group's extremes are shuffles within
-// them, so nothing passes through shared memory.
+// them, so nothing passes through shared memory.  A warp stays with one row and
+// keeps its rotation, page and norm weights in registers while it walks over the
+// heads, the next head's load under way.
+//
+// What bounds it: memory for many rows (16384 rows of 16 + 2 x 16 heads of 128,
+// bf16: 92 us, 4.5 TB/s of values read and written, next to ~130 instructions a
+// warp and step), the latency of seq -> page -> store for few.
 #include "paged.cuh"
 
 using namespace sm100;
 
 namespace {
 
+constexpr int kAppendWarps = 148 * 16;   // enough to keep the GPU's memory busy
+
 struct AppendParams {
   const void *qkv;
   const float *g_q, *g_k, *cos_t, *sin_t;
   const int32_t *pos, *seq;
   __nv_bfloat16 *q_out;
-  int64_t ld, items;   // items: T * (heads + 2 kv_heads)
-  int heads, rot, n_pos, pairs;
+  int64_t ld;
+  int T, heads, rot, n_pos, pairs;
+  int parts, steps;   // warps of a row, and a warp's steps
   float eps;
 };
 
@@ -34,12 +43,27 @@ __device__ __forceinline__ void load8(const float *p, float x[8]) {
   x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
 
-__device__ __forceinline__ void load8(const __nv_bfloat16 *p, float x[8]) {
-  const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// 8 values as they were loaded
+template <typename In>
+struct Raw;
+template <>
+struct Raw<__nv_bfloat16> {
+  uint4 v;
+  __device__ __forceinline__ void get(float x[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < 4; i++) x[2 * i] = bf16_lo(w[i]), x[2 * i + 1] = bf16_hi(w[i]);
-}
+    for (int i = 0; i < 4; i++) x[2 * i] = bf16_lo(w[i]), x[2 * i + 1] = bf16_hi(w[i]);
+  }
+};
+template <>
+struct Raw<float> {
+  float4 a, b;
+  __device__ __forceinline__ void get(float x[8]) const {
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  }
+};
+__device__ __forceinline__ Raw<__nv_bfloat16> load_raw(const __nv_bfloat16 *p) { return {ld_stream_u4(p)}; }
+__device__ __forceinline__ Raw<float> load_raw(const float *p) { return {ld_stream_f4(p), ld_stream_f4(p + 4)}; }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -95,110 +119,124 @@ __device__ __forceinline__ float sum_squares(const float x[8]) {
 #pragma unroll
       for (int i = 0; i < 8; i++) s[i] = shfl_add(s[i], 16);
     }
-    float lo = __fadd_rn(__fadd_rn(__fadd_rn(s[0], s[1]), s[2]), s[3]);
-    float hi = __fadd_rn(__fadd_rn(__fadd_rn(s[4], s[5]), s[6]), s[7]);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) lo = shfl_add(lo, o), hi = shfl_add(hi, o);
-    return __fadd_rn(lo, hi);
+    const float lo = __fadd_rn(__fadd_rn(__fadd_rn(s[0], s[1]), s[2]), s[3]);
+    const float hi = __fadd_rn(__fadd_rn(__fadd_rn(s[4], s[5]), s[6]), s[7]);
+    const bool up = threadIdx.x & 8;   // a lane goes on with its first runs, its partner with the second
+    const float got = __shfl_xor_sync(0xffffffffu, up ? lo : hi, 8);
+    float v = __fadd_rn(up ? hi : lo, got);
+    v = shfl_add(shfl_add(shfl_add(v, 4), 2), 1);
+    return shfl_add(v, 8);
   }
 }
 
+// A warp takes `steps` steps of 32 / (hd / 8) heads of one row: the row's place in
+// the cache, its rotation and the norm weights stay in registers.
 template <int HD, int BITS, typename In>
-__global__ void __launch_bounds__(256) paged_append_kernel(const PagedView c, const AppendParams a) {
-  constexpr int L = HD / 8;   // lanes of a head
+__global__ void __launch_bounds__(256, 4) paged_append_kernel(const PagedView c, const AppendParams a) {
+  constexpr int L = HD / 8, HPW = 32 / L;   // lanes of a head; heads of a warp's step
   pdl_trigger();
-  const int lane = threadIdx.x & 31, hl = lane % L;
-  int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
-  const bool live = item < a.items;
-  if (!live) item = a.items - 1;   // idle lanes follow the last head: the shuffles take whole warps
-  const int n_heads = a.heads + 2 * c.kv_heads;
-  const int64_t t = item / n_heads;
-  const int h = (int)(item - t * n_heads);
+  const int lane = threadIdx.x & 31, hl = lane % L, d0 = hl * 8;
+  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);   // (row, part of its heads)
+  if (item >= (int64_t)a.T * a.parts) return;
+  const int64_t t = item / a.parts;
+  const int n_heads = a.heads + 2 * c.kv_heads, h0 = (int)(item - t * a.parts) * a.steps * HPW;
   pdl_wait();
-  float x[8];
-  load8(static_cast<const In *>(a.qkv) + t * a.ld + (int64_t)h * HD + hl * 8, x);
+  const In *src = static_cast<const In *>(a.qkv) + t * a.ld + d0;
+  int h = h0 + lane / L;
+  Raw<In> next = load_raw(src + (int64_t)min(h, n_heads - 1) * HD);
   const int pos = a.pos[t], seq = a.seq[t];
-  const bool is_q = h < a.heads, turns = h < a.heads + c.kv_heads;
-  uint8_t *blk = paged_block(c, seq, pos);
-  const bool ok = blk != nullptr && (a.rot == 0 || pos < a.n_pos);
-  if (!ok && live && hl == 0) atomicOr(&g_paged_status, SM100_DECODE_ERR_ARG);
-  const float *g = is_q ? a.g_q : a.g_k;
-  const bool normed = turns && g != nullptr;
-  const float ss = sum_squares<HD>(x);
-  if (normed) {
-    const float r = rsqrtf(__fadd_rn(ss * (1.0f / HD), a.eps));
-    float w[8];
-    load8(g + hl * 8, w);
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
-  }
-  if (a.rot) {
-    const int half = a.rot / 2, d0 = hl * 8;
-    const bool in = turns && ok && d0 < a.rot;
+  const bool fits = a.rot == 0 || (pos >= 0 && pos < a.n_pos);
+  const int half = a.rot / 2;
+  const bool in = fits && d0 < a.rot, low = d0 < half;
+  float cs[8], sn[8], g[8];
+  if (in) {
     if (a.pairs) {
-      if (in) {
-        const float4 cs = __ldg(reinterpret_cast<const float4 *>(a.cos_t + (int64_t)pos * half + d0 / 2));
-        const float4 sn = __ldg(reinterpret_cast<const float4 *>(a.sin_t + (int64_t)pos * half + d0 / 2));
-        const float cc[4] = {cs.x, cs.y, cs.z, cs.w}, nn[4] = {sn.x, sn.y, sn.z, sn.w};
+      const float4 u = __ldg(reinterpret_cast<const float4 *>(a.cos_t + (int64_t)pos * half + d0 / 2));
+      const float4 w = __ldg(reinterpret_cast<const float4 *>(a.sin_t + (int64_t)pos * half + d0 / 2));
+      cs[0] = u.x, cs[1] = u.y, cs[2] = u.z, cs[3] = u.w;
+      sn[0] = w.x, sn[1] = w.y, sn[2] = w.z, sn[3] = w.w;
+    } else {   // x cos + (the other half's) (-sin, sin)
+      const int64_t at = (int64_t)pos * half + (low ? d0 : d0 - half);
+      load8(a.cos_t + at, cs);
+      load8(a.sin_t + at, sn);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float u = x[2 * i], w = x[2 * i + 1];
-          x[2 * i] = __fsub_rn(__fmul_rn(u, cc[i]), __fmul_rn(w, nn[i]));
-          x[2 * i + 1] = __fadd_rn(__fmul_rn(w, cc[i]), __fmul_rn(u, nn[i]));
-        }
-      }
-    } else {
-      const bool low = d0 < half;
-      const int src = d0 < a.rot ? (low ? lane + half / 8 : lane - half / 8) : lane;
-      float cc[8], nn[8];
-      if (in) {
-        const int64_t at = (int64_t)pos * half + (low ? d0 : d0 - half);
-        load8(a.cos_t + at, cc);
-        load8(a.sin_t + at, nn);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float y = __shfl_sync(0xffffffffu, x[i], src);
-        if (in) {
-          const float u = __fmul_rn(x[i], cc[i]), w = __fmul_rn(y, nn[i]);
-          x[i] = low ? __fsub_rn(u, w) : __fadd_rn(u, w);
-        }
-      }
+      for (int i = 0; i < 8; i++) sn[i] = low ? -sn[i] : sn[i];
     }
   }
-  if (is_q) {
-    if (live)
-      *reinterpret_cast<uint4 *>(a.q_out + (t * a.heads + h) * HD + hl * 8) = ok ? pack8(x) : make_uint4(0, 0, 0, 0);
-  }
-  const bool is_v = !turns;
-  const int kh = h - a.heads - (is_v ? c.kv_heads : 0);
+  uint8_t *blk = paged_block(c, seq, pos);
+  const bool ok = blk != nullptr && fits;
+  if (!ok && lane == 0) atomicOr(&g_paged_status, SM100_DECODE_ERR_ARG);
   const int row = pos & (c.page - 1);
-  const bool store = live && ok && !is_q;
-  uint8_t *dst = blk + (int64_t)kh * c.block + (is_v ? c.block / 2 : 0);
-  if constexpr (BITS == 16) {
-    if (store) *reinterpret_cast<uint4 *>(dst + ((int64_t)row * HD + hl * 8) * 2) = pack8(x);
-  } else {
-    float mn = x[0], mx = x[0];
+  const int partner = d0 < a.rot ? (low ? lane + half / 8 : lane - half / 8) : lane;
+  // this lane's part of the row's q, and of a key head's keys (values: half a block on)
+  __nv_bfloat16 *q_row = a.q_out + t * a.heads * HD + d0;
+  uint8_t *kv_row = blk + (BITS == 16 ? ((int64_t)row * HD + d0) * 2 : (int64_t)row * (HD / 2) + hl * 4);
+  const int marks = BITS == 16 ? 0 : (c.page - row) * (HD / 2) - hl * 4 + (row * (HD / kGroup) + hl / 8) * 4;
+  int kind = -1;   // whose norm weights g holds: 0 queries, 1 keys
+
+  for (int i = 0; i < a.steps && h0 + i * HPW < n_heads; i++, h += HPW) {
+    float x[8];
+    next.get(x);
+    if (h + HPW < n_heads) next = load_raw(src + (int64_t)(h + HPW) * HD);   // the next step's load under way
+    const bool live = h < n_heads, is_q = h < a.heads, turns = h < a.heads + c.kv_heads;
+    if (a.g_q || a.g_k) {
+      const float ss = sum_squares<HD>(x);
+      const float *gp = is_q ? a.g_q : a.g_k;
+      if (turns && gp) {
+        if (kind != !is_q) {
+          kind = !is_q;
+          load8(gp + d0, g);
+        }
+        const float r = rsqrtf(__fadd_rn(ss * (1.0f / HD), a.eps));
 #pragma unroll
-    for (int i = 1; i < 8; i++) mn = min_nan(mn, x[i]), mx = max_nan(mx, x[i]);
-#pragma unroll
-    for (int o = kGroup / 16; o > 0; o >>= 1) {   // the 8 lanes of a group
-      mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-      mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        for (int j = 0; j < 8; j++) x[j] = __fmul_rn(__fmul_rn(x[j], r), g[j]);
+      }
     }
-    const __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(__fsub_rn(mx, mn), 1.0f / 15.0f)), mb = __float2bfloat16_rn(mn);
-    const float s = __bfloat162float(sb), m = __bfloat162float(mb);
-    uint32_t codes = 0;
-    if (s > 0.0f) {
+    if (a.rot) {
+      if (a.pairs) {
+        if (in && turns) {
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-        codes |= (uint32_t)fminf(fmaxf(rintf((x[i] - m) / s), 0.0f), 15.0f) << (4 * i);
+          for (int j = 0; j < 4; j++) {
+            const float u = x[2 * j], w = x[2 * j + 1];
+            x[2 * j] = __fsub_rn(__fmul_rn(u, cs[j]), __fmul_rn(w, sn[j]));
+            x[2 * j + 1] = __fadd_rn(__fmul_rn(w, cs[j]), __fmul_rn(u, sn[j]));
+          }
+        }
+      } else if (h0 + i * HPW < a.heads + c.kv_heads) {   // one of the step's heads turns
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = __shfl_sync(0xffffffffu, x[j], partner);
+        if (in && turns) {
+#pragma unroll
+          for (int j = 0; j < 8; j++) x[j] = __fadd_rn(__fmul_rn(x[j], cs[j]), __fmul_rn(y[j], sn[j]));
+        }
+      }
     }
-    if (store) {
-      *reinterpret_cast<uint32_t *>(dst + (int64_t)row * (HD / 2) + hl * 4) = codes;
-      if (hl % 8 == 0) {
-        const __nv_bfloat162 pr = __halves2bfloat162(sb, mb);
-        *reinterpret_cast<__nv_bfloat162 *>(dst + (int64_t)c.page * (HD / 2) + ((int64_t)row * (HD / kGroup) + hl / 8) * 4) = pr;
+    if (is_q) *reinterpret_cast<uint4 *>(q_row + (int64_t)h * HD) = ok ? pack8(x) : make_uint4(0, 0, 0, 0);
+    const bool store = live && ok && !is_q;
+    uint8_t *dst = kv_row + (int64_t)(h - a.heads - (turns ? 0 : c.kv_heads)) * c.block + (turns ? 0 : c.block / 2);
+    if constexpr (BITS == 16) {
+      if (store) *reinterpret_cast<uint4 *>(dst) = pack8(x);
+    } else if (h0 + i * HPW + HPW > a.heads) {   // one of the step's heads is kept
+      float mn = x[0], mx = x[0];
+#pragma unroll
+      for (int j = 1; j < 8; j++) mn = min_nan(mn, x[j]), mx = max_nan(mx, x[j]);
+#pragma unroll
+      for (int o = kGroup / 16; o > 0; o >>= 1) {   // the 8 lanes of a group
+        mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      }
+      const __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(__fsub_rn(mx, mn), 1.0f / 15.0f)), mb = __float2bfloat16_rn(mn);
+      const float s = __bfloat162float(sb), m = __bfloat162float(mb);
+      uint32_t codes = 0;
+      if (s > 0.0f) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          codes |= (uint32_t)fminf(fmaxf(rintf((x[j] - m) / s), 0.0f), 15.0f) << (4 * j);
+      }
+      if (store) {
+        *reinterpret_cast<uint32_t *>(dst) = codes;
+        if (hl % 8 == 0) *reinterpret_cast<__nv_bfloat162 *>(dst + marks) = __halves2bfloat162(sb, mb);
       }
     }
   }
@@ -276,8 +314,14 @@ int sm100_paged_view(const Sm100PagedCache *c, const char *what, PagedView *v) {
 namespace {
 
 template <int HD>
-cudaError_t append_hd(const PagedView &v, int bits, int dtype, const AppendParams &p, cudaStream_t st) {
-  const int64_t blocks = (p.items * (HD / 8) + 255) / 256;
+cudaError_t append_hd(const PagedView &v, int bits, int dtype, AppendParams p, cudaStream_t st) {
+  // a row's heads in as few warps as still fill the GPU: 16384 rows of 48 heads in bf16 take 92 us with a warp a row, 104
+  // with ten steps a warp; 4093 rows of 36 heads in 4 bits (and their reading) 28.8 us with all steps in a warp, 45.9 with one
+  const int n_heads = p.heads + 2 * v.kv_heads, hpw = 32 / (HD / 8), all = (n_heads + hpw - 1) / hpw;
+  const int64_t even = (int64_t)p.T * all / kAppendWarps;
+  p.steps = (int)(even < 1 ? 1 : even < all ? even : all);
+  p.parts = (all + p.steps - 1) / p.steps;
+  const int64_t blocks = ((int64_t)p.T * p.parts + 7) / 8;
   const dim3 grid((unsigned)blocks), block(256);
   if (bits == 16)
     return dtype == SM100_DT_F32 ? launch_pdl(paged_append_kernel<HD, 16, float>, grid, block, 0, st, v, p)
@@ -308,9 +352,8 @@ extern "C" int sm100_paged_append(const Sm100PagedCache *c, const Sm100PagedAppe
     return sm100_set_error(SM100_ERR_ARG, "paged_append: row stride %lld of %lld elements, 16-byte rows and addresses",
                            (long long)ld, (long long)width);
   AppendParams p{a->qkv, a->g_q, a->g_k, a->cos_t, a->sin_t, a->pos, a->seq, static_cast<__nv_bfloat16 *>(a->q_out),
-                 ld, (int64_t)a->T * (a->heads + 2 * c->kv_heads), a->heads, rot ? a->rot : 0, a->n_pos, a->pairs,
-                 a->eps};
-  if (p.items * (c->head_dim / 8) / 256 >= INT32_MAX)
+                 ld, a->T, a->heads, rot ? a->rot : 0, a->n_pos, a->pairs, 0, 0, a->eps};
+  if ((int64_t)a->T * (a->heads + 2 * c->kv_heads) >= INT32_MAX)
     return sm100_set_error(SM100_ERR_ARG, "paged_append: %d rows in one call", a->T);
   cudaStream_t st = (cudaStream_t)stream;
   const cudaError_t e = c->head_dim == 64    ? append_hd<64>(v, c->bits, a->dtype, p, st)

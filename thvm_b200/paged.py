@@ -19,6 +19,8 @@ import ctypes
 
 from . import _lib as L
 
+_addressof = ctypes.addressof
+
 
 class Scratch:
     """The attention's workspace: grows to what its calls need."""
@@ -54,7 +56,12 @@ class PagedCache:
                                       bits, table.shape[0], table.shape[1])
         self._desc = ctypes.addressof(self.desc)
         self._raw_stream = torch._C._cuda_getCurrentRawStream
-        self._index = pool.device.index
+        self._device, self._index, self._n_seq = pool.device, pool.device.index, table.shape[0]
+        # what every call looks up
+        self._empty, self._bf16, self._f32, self._i32 = torch.empty, torch.bfloat16, torch.float32, torch.int32
+        self._rows = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16}
+        self._append, self._read, self._attention = (
+            self.lib.sm100_paged_append, self.lib.sm100_paged_read, self.lib.sm100_paged_attention)
         self._need: dict[tuple[int, int], int] = {}
 
     @classmethod
@@ -67,14 +74,14 @@ class PagedCache:
         table = torch.full((n_seq, max_pages), -1, dtype=torch.int32, device=device)
         return cls(pool, table, page, head_dim, bits, scratch)
 
-    def _int32(self, what: str, t, n: int):
-        if t.dtype != self.torch.int32 or t.device != self.pool.device or not t.is_contiguous() or t.numel() != n:
-            raise ValueError(f"{what} must be {n} dense int32 values beside the pool, got {t.dtype} {tuple(t.shape)}")
-        return t.data_ptr()
+    def _refuse(self, what: str, wanted: str, t):
+        raise ValueError(f"{what} must be {wanted} beside the pool, got {t.dtype} {tuple(t.shape)}"
+                         f"{'' if t.is_contiguous() else ' (strided)'} on {t.device}")
 
-    def _float(self, what: str, t, shape: tuple):
-        if t.dtype != self.torch.float32 or t.device != self.pool.device or not t.is_contiguous() or tuple(t.shape) != shape:
-            raise ValueError(f"{what} must be f32 {shape} beside the pool, got {t.dtype} {tuple(t.shape)}")
+    def _dense(self, what: str, t, dtype, n: int):
+        """The address of n dense values of dtype on the pool's GPU."""
+        if t.dtype is not dtype or t.get_device() != self._index or t.numel() != n or not t.is_contiguous():
+            self._refuse(what, f"{n} dense {dtype} values", t)
         return t.data_ptr()
 
     def append(self, qkv, pos, seq, heads: int, g_q=None, g_k=None, cos=None, sin=None, pairs: bool = False,
@@ -83,40 +90,47 @@ class PagedCache:
         or bf16, rows may be strided) at pos[t] of sequence seq[t]: norms and
         rotation of queries and keys, keys and values into the cache; returns
         the queries, bf16 [T, heads, head_dim] (sm100_paged_append)."""
-        torch, hd = self.torch, self.head_dim
+        hd, dense, i32, f32 = self.head_dim, self._dense, self._i32, self._f32
         T, width = qkv.shape
-        if qkv.dtype not in (torch.float32, torch.bfloat16) or width != (heads + 2 * self.kv_heads) * hd or \
-                qkv.device != self.pool.device or qkv.stride(1) != 1 or (T > 1 and qkv.stride(0) < width):
-            raise ValueError(f"qkv must be f32 or bf16 [T, {(heads + 2 * self.kv_heads) * hd}] beside the pool with "
-                             f"dense rows, got {qkv.dtype} {tuple(qkv.shape)}")
-        if (cos is None) != (sin is None):
-            raise ValueError("cos and sin come together")
+        step, one = qkv.stride()
+        dtype = self._rows.get(qkv.dtype)
+        if dtype is None or width != (heads + 2 * self.kv_heads) * hd or qkv.get_device() != self._index or one != 1 or \
+                (T > 1 and step < width):
+            self._refuse("qkv", f"f32 or bf16 [T, {(heads + 2 * self.kv_heads) * hd}] with dense rows", qkv)
         if out is None:
-            out = torch.empty(T, heads, hd, dtype=torch.bfloat16, device=qkv.device)
-        elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, heads, hd) or not out.is_contiguous() or \
-                out.device != self.pool.device:
-            raise ValueError(f"out must be dense bf16 {(T, heads, hd)}")
+            out = self._empty((T, heads, hd), dtype=self._bf16, device=self._device)
+            out_ptr = out.data_ptr()
+        else:
+            if tuple(out.shape) != (T, heads, hd):
+                self._refuse("out", f"{(T, heads, hd)}", out)
+            out_ptr = dense("out", out, self._bf16, T * heads * hd)
+        rot = n_pos = 0
+        cos_ptr = sin_ptr = None
+        if cos is not None or sin is not None:
+            if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape:
+                raise ValueError("cos and sin come together, f32 [n_pos, rot / 2]")
+            n_pos, half = cos.shape
+            rot = 2 * half
+            cos_ptr, sin_ptr = dense("cos", cos, f32, n_pos * half), dense("sin", sin, f32, n_pos * half)
         a = L.Sm100PagedAppendArgs(
-            qkv.data_ptr(), None if g_q is None else self._float("g_q", g_q, (hd,)),
-            None if g_k is None else self._float("g_k", g_k, (hd,)),
-            None if cos is None else self._float("cos", cos, (cos.shape[0], cos.shape[1])),
-            None if sin is None else self._float("sin", sin, tuple(cos.shape)), self._int32("pos", pos, T),
-            self._int32("seq", seq, T), out.data_ptr(), qkv.stride(0) if T > 1 else 0, T, heads,
-            L.DT_F32 if qkv.dtype == torch.float32 else L.DT_BF16, 0 if cos is None else 2 * cos.shape[1],
-            0 if cos is None else cos.shape[0], pairs, eps)
-        L.check(self.lib.sm100_paged_append(self._desc, ctypes.addressof(a), self._raw_stream(self._index)),
-                "paged_append")
+            qkv.data_ptr(), None if g_q is None else dense("g_q", g_q, f32, hd),
+            None if g_k is None else dense("g_k", g_k, f32, hd), cos_ptr, sin_ptr, dense("pos", pos, i32, T),
+            dense("seq", seq, i32, T), out_ptr, step if T > 1 else 0, T, heads, dtype, rot, n_pos, pairs, eps)
+        rc = self._append(self._desc, _addressof(a), self._raw_stream(self._index))
+        if rc:
+            L.check(rc, "paged_append")
         return out
 
     def read(self, pos, seq):
         """(keys, values), bf16 [T, kv_heads, head_dim], of token pos[t] of
         sequence seq[t] (sm100_paged_read)."""
-        torch = self.torch
         T = pos.numel()
-        k = torch.empty(T, self.kv_heads, self.head_dim, dtype=torch.bfloat16, device=self.pool.device)
-        v = torch.empty_like(k)
-        L.check(self.lib.sm100_paged_read(self._desc, self._int32("pos", pos, T), self._int32("seq", seq, T),
-                                          k.data_ptr(), v.data_ptr(), T, self._raw_stream(self._index)), "paged_read")
+        both = self._empty((2, T, self.kv_heads, self.head_dim), dtype=self._bf16, device=self._device)
+        k, v = both.unbind(0)
+        rc = self._read(self._desc, self._dense("pos", pos, self._i32, T), self._dense("seq", seq, self._i32, T),
+                        k.data_ptr(), v.data_ptr(), T, self._raw_stream(self._index))
+        if rc:
+            L.check(rc, "paged_read")
         return k, v
 
     def attend(self, q, kv_len, q_off=None, max_rows: int = 1, scale: float | None = None, out=None):
@@ -124,30 +138,35 @@ class PagedCache:
         bf16 [T, heads, head_dim].  kv_len [n_seq] counts the cached tokens, the
         new ones among them; sequence s has the rows q_off[s] .. q_off[s + 1] - 1
         (at most max_rows), without q_off row s alone (sm100_paged_attention)."""
-        torch, hd = self.torch, self.head_dim
+        hd, dense, i32 = self.head_dim, self._dense, self._i32
         T, heads, d = q.shape
-        if q.dtype != torch.bfloat16 or d != hd or q.device != self.pool.device or q.stride(2) != 1 or \
-                (heads > 1 and q.stride(1) != hd) or (T > 1 and q.stride(0) < heads * hd):
-            raise ValueError(f"q must be bf16 [T, heads, {hd}] beside the pool with dense rows, got {q.dtype} {tuple(q.shape)}")
+        step, head, one = q.stride()
+        if q.dtype is not self._bf16 or d != hd or q.get_device() != self._index or one != 1 or \
+                (heads > 1 and head != hd) or (T > 1 and step < heads * hd):
+            self._refuse("q", f"bf16 [T, heads, {hd}] with dense rows", q)
         if out is None:
-            out = torch.empty(T, heads, hd, dtype=torch.bfloat16, device=q.device)
-        elif out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous() or \
-                out.device != self.pool.device:
-            raise ValueError(f"out must be dense bf16 {tuple(q.shape)}")
-        n_seq = self.table.shape[0]
+            out = self._empty((T, heads, hd), dtype=self._bf16, device=self._device)
+            out_ptr = out.data_ptr()
+        else:
+            if out.shape != q.shape:
+                self._refuse("out", f"{tuple(q.shape)}", out)
+            out_ptr = dense("out", out, self._bf16, T * heads * hd)
         need = self._need.get((heads, max_rows))
         if need is None:
             need = int(self.lib.sm100_paged_attention_ws_bytes(self._desc, heads, max_rows))
             if not need:
                 raise ValueError(f"heads {heads} (a multiple of {self.kv_heads}), max_rows {max_rows}")
             self._need[heads, max_rows] = need
-        ws = self.scratch.take(need, self.pool.device)
-        a = L.Sm100PagedAttnArgs(q.data_ptr(), self._int32("kv_len", kv_len, n_seq),
-                                 None if q_off is None else self._int32("q_off", q_off, n_seq + 1), out.data_ptr(),
-                                 ws.ptr, ws.nbytes, q.stride(0) if T > 1 else 0, T, heads, max_rows,
+        ws = self.scratch
+        if need > ws.nbytes:
+            ws.take(need, self._device)
+        a = L.Sm100PagedAttnArgs(q.data_ptr(), dense("kv_len", kv_len, i32, self._n_seq),
+                                 None if q_off is None else dense("q_off", q_off, i32, self._n_seq + 1), out_ptr,
+                                 ws.ptr, ws.nbytes, step if T > 1 else 0, T, heads, max_rows,
                                  hd ** -0.5 if scale is None else scale)
-        L.check(self.lib.sm100_paged_attention(self._desc, ctypes.addressof(a), self._raw_stream(self._index)),
-                "paged_attention")
+        rc = self._attention(self._desc, _addressof(a), self._raw_stream(self._index))
+        if rc:
+            L.check(rc, "paged_attention")
         return out
 
     def status(self) -> int:
