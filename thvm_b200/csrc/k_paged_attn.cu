@@ -15,8 +15,9 @@
 // CTA that arrives last at the unit's counter joins them in CTA order (no
 // order of arrival enters the result).
 //
-// A CTA: one warp brings tiles in by bulk copies (a page of a key head is one
-// contiguous block: one copy) through a ring of stages; NW warps take 16 of a
+// A CTA: one warp brings tiles in by bulk copies (a page's keys, values and
+// their marks, each area of the tile's pages end to end, so that every place in
+// a tile is a constant) through a ring of stages; four warps take a quarter of a
 // tile's tokens each, with a running maximum and sum of their own, joined when
 // the unit ends.
 //
@@ -35,7 +36,8 @@
 // applied outside: S = s * (Q . (128 + c)) + (m - 128 s) * sum Q per group of 64
 // dimensions, and p * s per token is V's weight, sum p (m - 16 s) its shift.
 // Weights enter as bf16 hi + lo, so their rounding (2^-17) is far below the
-// output's.
+// output's; with up to 4 query columns the low parts are columns 4 to 7 of the
+// same product.
 #include "paged.cuh"
 #include "tma.cuh"
 
@@ -56,18 +58,24 @@ struct AttnParams {
 
 constexpr int kMaxPieces = 148 * 4;   // CTAs of a launch at most
 
-template <int HD, int BITS, int NT>
+// COLS query columns a unit: 4 (4 bits only: the weights' low parts take the
+// other half of the 8 columns of a product), 8 or 16.
+template <int HD, int BITS, int COLS>
 struct Shape {
   static constexpr int NW = 4;                                  // warps at the products
   static constexpr int KS = BITS == 4 || HD == 64 ? 2 : 1;      // 16-token steps that a warp takes of a tile
   static constexpr int TS = 16 * KS * NW;                       // tokens of a tile
-  static constexpr int TOKEN = BITS == 4 ? HD / 2 + HD / kGroup * 4 : 2 * HD;
-  static constexpr int TILE = 2 * TS * TOKEN;                   // bytes of a tile
-  static constexpr int NC = 8 * NT;                             // query columns
-  static constexpr int CHUNK = 16;                              // accumulators joined at a time
-  static constexpr int ACC = HD / 16 * NT * 4;                  // accumulators of a thread
-  static constexpr int PART = ACC * 32 + 2 * NC;                // floats of a unit's part
-  static constexpr int RED = NW * CHUNK * 32 * 4;
+  static constexpr int GR = HD / kGroup;
+  static constexpr int ROW = BITS == 4 ? HD / 2 : 2 * HD;       // bytes of a token's keys
+  static constexpr int MARKS = BITS == 4 ? 4 * GR : 0;          // and of their scales and minima
+  // a tile in shared memory: keys, their marks, values, their marks of all tokens
+  static constexpr int V = TS * (ROW + MARKS), TILE = 2 * V;
+  static constexpr bool DUAL = COLS == 4;
+  static constexpr int NT = COLS == 16 ? 2 : 1;                 // column tiles of 8
+  static constexpr int ACC = HD / 16 * NT;                      // accumulator tiles (4 floats) of a thread
+  static constexpr int CHUNK = 4;                               // of them joined at a time, one a warp
+  static constexpr int PART = ACC * 128 + 2 * COLS;             // floats of a unit's part
+  static constexpr int RED = NW * CHUNK * 512;
   // CTAs of an SM: what the registers leave (5 warps each: 128 registers at 3, 168 at 2)
   static constexpr int CTAS = HD == 256 ? (BITS == 4 ? 2 : 1) : NT == 2 || (HD == 128 && BITS == 16) ? 2 : 3;
   static constexpr int ROOM = 227 * 1024 / CTAS - RED - 3072;
@@ -105,6 +113,11 @@ __device__ __forceinline__ void split_weights(float w0, float w1, uint32_t &hi, 
   const uint32_t h = pack2(w0, w1);
   hi = transpose8x8(h);
   lo = transpose8x8(pack2(w0 - bf16_lo(h), w1 - bf16_hi(h)));
+}
+// the same with the low parts in columns 4 .. 7, which repeat columns 0 .. 3
+__device__ __forceinline__ uint32_t split_columns(float w0, float w1, bool low) {
+  const uint32_t h = pack2(w0, w1), l = pack2(w0 - bf16_lo(h), w1 - bf16_hi(h));
+  return transpose8x8(low ? l : h);
 }
 
 // (x & mask) | bits as the one instruction that it is (written plainly it became two, a third of a step's instructions)
@@ -230,16 +243,27 @@ struct Line {
   }
 };
 
-template <int HD, int BITS, int NT>
-__global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, BITS, NT>::CTAS)
+// Waits for a free stage: the copies' warp has time, and a busy wait would take issue slots from the products.
+__device__ __forceinline__ bool wait_free(uint64_t *bar, uint32_t parity) {
+  for (uint32_t i = 0; i < (1u << 22); i++) {
+    if (mbar_try_wait(bar, parity)) return true;
+    __nanosleep(64);
+  }
+  atomicOr(&g_paged_status, SM100_DECODE_ERR_STALL);
+  return false;
+}
+
+template <int HD, int BITS, int COLS>
+__global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD, BITS, COLS>::CTAS)
     paged_attn_kernel(const __grid_constant__ PagedView c, const __grid_constant__ AttnParams a) {
-  using S = Shape<HD, BITS, NT>;
-  constexpr int NW = S::NW, KS = S::KS, TS = S::TS, NC = S::NC, STAGES = S::STAGES, GR = HD / kGroup;
+  using S = Shape<HD, BITS, COLS>;
+  constexpr int NW = S::NW, KS = S::KS, TS = S::TS, NT = S::NT, STAGES = S::STAGES, GR = S::GR, ROW = S::ROW, MARKS = S::MARKS;
+  constexpr bool DUAL = S::DUAL;
   extern __shared__ __align__(128) uint8_t smem[];
-  float *red = reinterpret_cast<float *>(smem + STAGES * S::TILE);
+  float4 *red = reinterpret_cast<float4 *>(smem + STAGES * S::TILE);
   __shared__ uint64_t full[STAGES], empty[STAGES];
   __shared__ uint16_t valid[STAGES][TS / 16];
-  __shared__ float wm[NW][NC], wl[NW][NC], um[NC], ul[NC];
+  __shared__ float wm[NW][COLS], wl[NW][COLS], um[COLS], ul[COLS];
   __shared__ uint32_t arrived;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_trigger();
@@ -252,7 +276,7 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
   }
   __syncthreads();
   pdl_wait();
-  Line<TS, NC> line;
+  Line<TS, COLS> line;
   line.a = &a;
   line.c = &c;
   const int me = blockIdx.x;
@@ -262,36 +286,40 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
   uint32_t it = 0;   // tiles through the ring
 
   if (warp == NW) {
-    // ---- the copies
+    // ---- the copies: a lane takes one of a page's areas (keys, their marks, values, their marks)
+    constexpr int AREAS = BITS == 4 ? 4 : 2;
+    const int area = lane % AREAS, in_tile = lane / AREAS, page = c.page;
+    const bool is_v = area >= AREAS / 2, is_marks = BITS == 4 && (area & 1);
+    const uint32_t bytes = page * (is_marks ? MARKS : ROW);
+    const uint32_t from = (is_v ? c.block / 2 : 0) + (is_marks ? page * ROW : 0);
+    uint8_t *to = smem + (is_v ? S::V : 0) + (is_marks ? TS * ROW : 0) + in_tile * bytes;
     const int per = TS >> c.page_log2;            // pages of a tile
-    const uint32_t block = c.block;
     const uint64_t pol = policy_evict_first();
     bool ok_ring = true;
     for (;;) {
       line.span(w0, w1, t0, t1);
       for (int t = t0; t < t1 && ok_ring; t++, it++) {
         const int st = it % STAGES;
-        const int slot = t * per + lane, key = slot << c.page_log2;
+        const int slot = t * per + in_tile, key = slot << c.page_log2;
         int id = -1;
-        bool want = lane < per && key < line.len;
+        const bool want = in_tile < per && key < line.len;
         if (want) id = c.table[(int64_t)line.s * c.max_pages + slot];
         const bool ok = want && (unsigned)id < (unsigned)c.n_pages;
         if (want && !ok) atomicOr(&g_paged_status, SM100_DECODE_ERR_ARG);
         const uint32_t oks = __ballot_sync(0xffffffffu, ok);
-        if (it >= STAGES && !mbar_wait(&empty[st], (it / STAGES - 1) & 1, &g_paged_status, false)) {
+        if (it >= STAGES && !wait_free(&empty[st], (it / STAGES - 1) & 1)) {
           ok_ring = false;
           break;
         }
         if (lane < TS / 16) {
           const int base = t * TS + 16 * lane, n = min(max(line.len - base, 0), 16);
-          valid[st][lane] = oks >> ((16 * lane) >> c.page_log2) & 1 ? (uint16_t)((1u << n) - 1) : 0;
+          valid[st][lane] = oks >> (((16 * lane) >> c.page_log2) * AREAS) & 1 ? (uint16_t)((1u << n) - 1) : 0;
         }
         __syncwarp();
-        if (lane == 0) mbar_expect_tx(&full[st], __popc(oks) * block);
+        if (lane == 0) mbar_expect_tx(&full[st], __popc(oks) / AREAS * c.block);
         __syncwarp();
         if (ok)
-          bulk_g2s_hint(smem + st * S::TILE + lane * block,
-                        c.pool + ((int64_t)id * c.kv_heads + line.h) * block, block, &full[st], pol);
+          bulk_g2s_hint(to + st * S::TILE, c.pool + ((int64_t)id * c.kv_heads + line.h) * c.block + from, bytes, &full[st], pol);
       }
       if (!ok_ring || line.at + kPad + line.tiles >= w1) break;
       line.next();
@@ -305,17 +333,22 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
 
   // ---- the products
   const int g = lane >> 2, cq = lane & 3;
+  const auto column = [](int col) { return DUAL ? col & 3 : col; };   // the query column of a product's column
+  // this thread's places in a tile: tokens g, g + 8 of the keys; 2 cq, 2 cq + 1 and 8 on of the values
+  const uint8_t *kp = smem + (16 * KS * warp + g) * ROW + (BITS == 4 ? cq * 8 : cq * 16);
+  const uint8_t *vp = smem + S::V + (16 * KS * warp + 2 * cq) * ROW + (BITS == 4 ? g * 4 : g * 16);
+  const uint8_t *mp = smem + TS * ROW + (16 * KS * warp + g) * MARKS;   // marks of tokens g, g + 8 (values': V on)
   bool stalled = false;
   for (;; line.next()) {
     line.span(w0, w1, t0, t1);
     if (t0 >= t1) break;   // the piece ends before the unit's first tile
-    const int n_cols = min(NC, line.rows * a.group - line.ct * NC);
+    const int n_cols = min(COLS, line.rows * a.group - line.ct * COLS);
     // Q^T fragments: column g of each 8, this lane's dimensions
     uint32_t qf[NT][HD / 8];
     float qs[GR][NT][2];   // 4 bits: sum of a column's queries over a group (columns 2 cq, 2 cq + 1)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      const int col = nt * 8 + g, at = line.ct * NC + col;
+      const int col = column(nt * 8 + g), at = line.ct * COLS + col;
       const __nv_bfloat16 *src = a.q + (int64_t)(line.first + at / a.group) * a.ld_q +
                                  (int64_t)(line.h * a.group + at % a.group) * HD;
       uint4 v[HD / 32];
@@ -354,10 +387,10 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        const int col = nt * 8 + 2 * cq + e, at = line.ct * NC + col;
+        const int col = column(nt * 8 + 2 * cq + e), at = line.ct * COLS + col;
         lim[nt][e] = col < n_cols ? line.len - line.rows + at / a.group + 1 : 0;
       }
-    const int row0 = line.ct * NC / a.group, row1 = (line.ct * NC + n_cols - 1) / a.group;
+    const int row0 = line.ct * COLS / a.group, row1 = (line.ct * COLS + n_cols - 1) / a.group;
     const int lim_min = line.len - line.rows + row0 + 1;
     float o[GR * 4][NT][4], l[NT][2], m[NT][2], z[GR][NT][2];
 #pragma unroll
@@ -383,34 +416,25 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
 #pragma unroll
       for (int x = 0; x < KS; x++) any_bits |= bits[x] = stalled ? 0 : valid[st][KS * warp + x];
       if (any_bits != 0) {
-        // this warp's tokens: KS steps of 16, each inside a page's block
-        const uint8_t *kb[KS];
-        int row_in[KS], key0[KS];
+        const int in_ring = st * S::TILE;
+        const uint8_t *kt = kp + in_ring, *vt = vp + in_ring, *mt = mp + in_ring;
+        const int key0 = t * TS + 16 * KS * warp;
         float sc[KS][NT][4];
-        bool edge[KS];
 #pragma unroll
-        for (int x = 0; x < KS; x++) {
-          const int at = 16 * (KS * warp + x);
-          kb[x] = smem + st * S::TILE + (at >> c.page_log2) * c.block;
-          row_in[x] = at & (c.page - 1);
-          key0[x] = t * TS + at;
-          edge[x] = bits[x] != 0xffffu || key0[x] + 16 > lim_min;
+        for (int x = 0; x < KS; x++)
 #pragma unroll
           for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int e = 0; e < 4; e++) sc[x][nt][e] = 0.0f;
-        }
         if constexpr (BITS == 4) {
 #pragma unroll
           for (int gr = 0; gr < GR; gr++)
 #pragma unroll
             for (int x = 0; x < KS; x++) {
-              const uint8_t *km = kb[x] + c.page * (HD / 2) + (row_in[x] + g) * (GR * 4) + gr * 4;
-              const uint8_t *kc = kb[x] + (row_in[x] + g) * (HD / 2) + cq * 8 + gr * 32;
-              const uint2 u0 = *reinterpret_cast<const uint2 *>(kc);
-              const uint2 u8 = *reinterpret_cast<const uint2 *>(kc + 8 * (HD / 2));
-              const uint32_t m0 = *reinterpret_cast<const uint32_t *>(km);
-              const uint32_t m8 = *reinterpret_cast<const uint32_t *>(km + 8 * (GR * 4));
+              const uint2 u0 = *reinterpret_cast<const uint2 *>(kt + x * 16 * ROW + gr * 32);
+              const uint2 u8 = *reinterpret_cast<const uint2 *>(kt + x * 16 * ROW + 8 * ROW + gr * 32);
+              const uint32_t m0 = *reinterpret_cast<const uint32_t *>(mt + x * 16 * MARKS + gr * 4);
+              const uint32_t m8 = *reinterpret_cast<const uint32_t *>(mt + x * 16 * MARKS + 8 * MARKS + gr * 4);
               float acc[NT][4];
 #pragma unroll
               for (int nt = 0; nt < NT; nt++)
@@ -439,9 +463,8 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
           for (int i = 0; i < HD / 32; i++)
 #pragma unroll
             for (int x = 0; x < KS; x++) {
-              const uint8_t *kc = kb[x] + (row_in[x] + g) * (2 * HD) + cq * 16 + i * 64;
-              const uint4 x0 = *reinterpret_cast<const uint4 *>(kc);
-              const uint4 x8 = *reinterpret_cast<const uint4 *>(kc + 8 * (2 * HD));
+              const uint4 x0 = *reinterpret_cast<const uint4 *>(kt + x * 16 * ROW + i * 64);
+              const uint4 x8 = *reinterpret_cast<const uint4 *>(kt + x * 16 * ROW + 8 * ROW + i * 64);
               const uint32_t a0[4] = {x0.x, x8.x, x0.y, x8.y}, a1[4] = {x0.z, x8.z, x0.w, x8.w};
 #pragma unroll
               for (int nt = 0; nt < NT; nt++) {
@@ -450,17 +473,21 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
               }
             }
         }
+        // tokens that a column does not see, or that are not there
+        bool edge = key0 + 16 * KS > lim_min;
 #pragma unroll
-        for (int x = 0; x < KS; x++)
-          if (edge[x]) {
+        for (int x = 0; x < KS; x++) edge |= bits[x] != 0xffffu;
+        if (edge) {
+#pragma unroll
+          for (int x = 0; x < KS; x++)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
               for (int e = 0; e < 4; e++) {
                 const int r = e < 2 ? g : g + 8;
-                if (!(bits[x] >> r & 1) || key0[x] + r >= lim[nt][e & 1]) sc[x][nt][e] = -INFINITY;
+                if (!(bits[x] >> r & 1) || key0 + 16 * x + r >= lim[nt][e & 1]) sc[x][nt][e] = -INFINITY;
               }
-          }
+        }
         // the running maximum moves only where a column grows past it by 2^8 (a weight of up to 2^8 costs an f32 sum
         // nothing): most tiles then skip the reduction and the rescaling
         float top[NT][2];
@@ -503,39 +530,46 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
               l[nt][e] += sc[x][nt][e] + sc[x][nt][2 + e];
             }
           }
-        const int k0 = 2 * cq;   // this lane's tokens of V^T: k0, k0 + 1, k0 + 8, k0 + 9
         if constexpr (BITS == 4) {
 #pragma unroll
           for (int gr = 0; gr < GR; gr++)
 #pragma unroll
             for (int x = 0; x < KS; x++) {
-              const uint8_t *vb = kb[x] + c.block / 2;
-              const uint8_t *vm = vb + c.page * (HD / 2) + (row_in[x] + g) * (GR * 4) + gr * 4;
-              vb += (row_in[x] + k0) * (HD / 2) + g * 4 + gr * 32;
-              const uint32_t m0 = *reinterpret_cast<const uint32_t *>(vm);
-              const uint32_t m8 = *reinterpret_cast<const uint32_t *>(vm + 8 * (GR * 4));
-              const uint32_t wa = *reinterpret_cast<const uint32_t *>(vb);
-              const uint32_t wb = *reinterpret_cast<const uint32_t *>(vb + (HD / 2));
-              const uint32_t wc = *reinterpret_cast<const uint32_t *>(vb + 8 * (HD / 2));
-              const uint32_t wd = *reinterpret_cast<const uint32_t *>(vb + 9 * (HD / 2));
+              const uint8_t *vc = vt + x * 16 * ROW + gr * 32;
+              const uint32_t m0 = *reinterpret_cast<const uint32_t *>(mt + S::V + x * 16 * MARKS + gr * 4);
+              const uint32_t m8 = *reinterpret_cast<const uint32_t *>(mt + S::V + x * 16 * MARKS + 8 * MARKS + gr * 4);
+              const uint32_t wa = *reinterpret_cast<const uint32_t *>(vc);
+              const uint32_t wb = *reinterpret_cast<const uint32_t *>(vc + ROW);
+              const uint32_t wc = *reinterpret_cast<const uint32_t *>(vc + 8 * ROW);
+              const uint32_t wd = *reinterpret_cast<const uint32_t *>(vc + 9 * ROW);
               const float s0 = bf16_lo(m0), s8 = bf16_lo(m8);
               const float b0 = fmaf(-16.0f, s0, bf16_hi(m0)), b8 = fmaf(-16.0f, s8, bf16_hi(m8));
               uint32_t p0[NT], p8[NT], r0[NT], r8[NT];
 #pragma unroll
               for (int nt = 0; nt < NT; nt++) {
                 float w[4];
+                if (!edge) {
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                  w[e] = sc[x][nt][e] * s0, w[2 + e] = sc[x][nt][2 + e] * s8;
-                  float d0 = sc[x][nt][e] * b0, d8 = sc[x][nt][2 + e] * b8;
-                  if (edge[x]) {   // a weight of zero leaves out whatever the token holds
-                    if (sc[x][nt][e] == 0.0f) w[e] = d0 = 0.0f;
-                    if (sc[x][nt][2 + e] == 0.0f) w[2 + e] = d8 = 0.0f;
+                  for (int e = 0; e < 2; e++) {
+                    w[e] = sc[x][nt][e] * s0, w[2 + e] = sc[x][nt][2 + e] * s8;
+                    z[gr][nt][e] = fmaf(sc[x][nt][e], b0, fmaf(sc[x][nt][2 + e], b8, z[gr][nt][e]));
                   }
-                  z[gr][nt][e] += d0 + d8;
+                } else {   // a weight of zero leaves out whatever the token holds
+#pragma unroll
+                  for (int e = 0; e < 2; e++) {
+                    const bool k0 = sc[x][nt][e] != 0.0f, k8 = sc[x][nt][2 + e] != 0.0f;
+                    w[e] = k0 ? sc[x][nt][e] * s0 : 0.0f, w[2 + e] = k8 ? sc[x][nt][2 + e] * s8 : 0.0f;
+                    if (k0) z[gr][nt][e] += sc[x][nt][e] * b0;
+                    if (k8) z[gr][nt][e] += sc[x][nt][2 + e] * b8;
+                  }
                 }
-                split_weights(w[0], w[1], p0[nt], r0[nt]);
-                split_weights(w[2], w[3], p8[nt], r8[nt]);
+                if constexpr (DUAL) {
+                  p0[nt] = split_columns(w[0], w[1], cq >= 2);
+                  p8[nt] = split_columns(w[2], w[3], cq >= 2);
+                } else {
+                  split_weights(w[0], w[1], p0[nt], r0[nt]);
+                  split_weights(w[2], w[3], p8[nt], r8[nt]);
+                }
               }
               const uint32_t lo[2] = {__byte_perm(wa, wb, 0x5410), __byte_perm(wa, wb, 0x7632)};
               const uint32_t hi[2] = {__byte_perm(wc, wd, 0x5410), __byte_perm(wc, wd, 0x7632)};
@@ -547,15 +581,15 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                   mma_bf16(o[4 * gr + j][nt], af, p0[nt], p8[nt]);
-                  mma_bf16(o[4 * gr + j][nt], af, r0[nt], r8[nt]);
+                  if constexpr (!DUAL) mma_bf16(o[4 * gr + j][nt], af, r0[nt], r8[nt]);
                 }
               }
             }
         } else {
-          const int tk[4] = {k0, k0 + 1, k0 + 8, k0 + 9};
+          const int k0 = 2 * cq, tk[4] = {k0, k0 + 1, k0 + 8, k0 + 9};
 #pragma unroll
           for (int x = 0; x < KS; x++) {
-            const uint8_t *vb = kb[x] + c.block / 2 + (row_in[x] + k0) * (2 * HD) + g * 16;
+            const uint8_t *vc = vt + x * 16 * ROW;
             uint32_t p0[NT], p8[NT], r0[NT], r8[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
@@ -566,8 +600,8 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
             for (int gr = 0; gr < GR; gr++) {
               uint4 v[4];
 #pragma unroll
-              for (int k = 0; k < 4; k++) v[k] = *reinterpret_cast<const uint4 *>(vb + gr * 128 + (tk[k] - k0) * (2 * HD));
-              if (!edge[x]) {
+              for (int k = 0; k < 4; k++) v[k] = *reinterpret_cast<const uint4 *>(vc + gr * 128 + (k >> 1) * 8 * ROW + (k & 1) * ROW);
+              if (!edge) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                   const uint32_t wa = (&v[0].x)[j], wb = (&v[1].x)[j], wc = (&v[2].x)[j], wd = (&v[3].x)[j];
@@ -587,7 +621,7 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
                   uint32_t keep[4];
 #pragma unroll
                   for (int k = 0; k < 4; k++)
-                    keep[k] = (bits[x] >> tk[k] & 1) && key0[x] + tk[k] < seen ? 0xffffffffu : 0u;
+                    keep[k] = (bits[x] >> tk[k] & 1) && key0 + 16 * x + tk[k] < seen ? 0xffffffffu : 0u;
 #pragma unroll
                   for (int j = 0; j < 4; j++) {
                     const uint32_t wa = (&v[0].x)[j] & keep[0], wb = (&v[1].x)[j] & keep[1];
@@ -615,6 +649,7 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
     }
 
     // ---- the warps' parts of the unit joined
+    const bool mine = !DUAL || cq < 2;   // this thread's columns are query columns
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -627,7 +662,7 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
             for (int gr = 0; gr < GR; gr++) z[gr][nt][e] += __shfl_xor_sync(0xffffffffu, z[gr][nt][e], x);
           }
         }
-        if (g == 0) wm[warp][nt * 8 + 2 * cq + e] = m[nt][e], wl[warp][nt * 8 + 2 * cq + e] = l[nt][e];
+        if (g == 0 && mine) wm[warp][nt * 8 + 2 * cq + e] = m[nt][e], wl[warp][nt * 8 + 2 * cq + e] = l[nt][e];
       }
     const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory"); };
     sync();
@@ -636,68 +671,66 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        const int col = nt * 8 + 2 * cq + e;
+        const int col = column(nt * 8 + 2 * cq + e);
         float top = -INFINITY, sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < NW; i++) top = fmaxf(top, wm[i][col]);
 #pragma unroll
         for (int i = 0; i < NW; i++) sum += wm[i][col] == -INFINITY ? 0.0f : wl[i][col] * ex2(wm[i][col] - top);
         f[nt][e] = m[nt][e] == -INFINITY ? 0.0f : ex2(m[nt][e] - top);
-        if (warp == 0 && g == 0) um[col] = top, ul[col] = sum;
+        if (warp == 0 && g == 0 && mine) um[col] = top, ul[col] = sum;
       }
     // where the piece ends inside the unit, or began inside it: a part
     const bool whole = t0 == 0 && t1 == line.tiles;
     float *part = a.parts + ((int64_t)me * 2 + (t0 == 0)) * S::PART;
-      const auto put = [&](int i, int nt, int e, float v0, float v1) {   // dimensions d, d + 1 of a column
-      const int col = nt * 8 + 2 * cq + e, at = line.ct * NC + col;
-      if (col >= n_cols) return;
+    // an accumulator tile's values: dimensions d, d + 1 of columns 2 cq, 2 cq + 1
+    const auto put = [&](int i, int nt, float4 v) {
       const int d = (i >> 2) * 64 + 8 * g + 2 * (i & 3);
-      const float inv = ul[col] > 0.0f ? 1.0f / ul[col] : ul[col] == 0.0f ? 0.0f : ul[col];
-      *reinterpret_cast<uint32_t *>(a.out + ((int64_t)(line.first + at / a.group) * a.heads + line.h * a.group + at % a.group) * HD + d) =
-          pack2(v0 * inv, v1 * inv);
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int col = nt * 8 + 2 * cq + e, at = line.ct * COLS + col;
+        if (!mine || col >= n_cols) continue;
+        const float inv = ul[col] > 0.0f ? 1.0f / ul[col] : ul[col] == 0.0f ? 0.0f : ul[col];
+        *reinterpret_cast<uint32_t *>(a.out + ((int64_t)(line.first + at / a.group) * a.heads + line.h * a.group + at % a.group) * HD + d) =
+            e ? pack2(v.y * inv, v.w * inv) : pack2(v.x * inv, v.z * inv);
+      }
     };
-    constexpr int CI = S::CHUNK / (4 * NT);   // accumulator tiles of a chunk
+    const bool used = mine && 2 * cq < n_cols;   // a lane without query columns has nothing to join (its low parts are added)
+    for (bool last = whole;; last = true) {
 #pragma unroll
-    for (int ch = 0; ch < GR * 4 / CI; ch++) {
+      for (int ch = 0; ch < S::ACC / S::CHUNK; ch++) {
 #pragma unroll
-      for (int k = 0; k < CI; k++)
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int k = 0; k < S::CHUNK; k++) {
+          const int i = (ch * S::CHUNK + k) / NT, nt = (ch * S::CHUNK + k) % NT;
+          float v[4];
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const int i = ch * CI + k;
-            float v = o[i][nt][e];
-            if constexpr (BITS == 4) v += z[i >> 2][nt][e & 1];
-            v = f[nt][e & 1] == 0.0f ? 0.0f : v * f[nt][e & 1];
-            red[(warp * S::CHUNK + (k * NT + nt) * 4 + e) * 32 + lane] = v;
+            v[e] = o[i][nt][e];
+            if constexpr (DUAL) v[e] += __shfl_xor_sync(0xffffffffu, v[e], 2);
+            if constexpr (BITS == 4) v[e] += z[i >> 2][nt][e & 1];
+            v[e] = f[nt][e & 1] == 0.0f ? 0.0f : v[e] * f[nt][e & 1];
           }
-      sync();
-      // pairs of accumulators (e, e + 2), two neighbouring dimensions of a column, over the warps
-#pragma unroll
-      for (int y = 0; y < S::CHUNK / 2 / NW + (S::CHUNK / 2 % NW != 0); y++) {
-        const int pr = y * NW + warp;
-        if (pr < S::CHUNK / 2) {
-          const int e = pr & 1, tile = pr >> 1, k = tile / NT, nt = tile % NT;
-          float v0 = 0.0f, v1 = 0.0f;
+          if (used) red[(warp * S::CHUNK + k) * 32 + lane] = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        sync();
+        if (used) {
+          const int at = ch * S::CHUNK + warp;   // a warp's tile, over the warps
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
           for (int x = 0; x < NW; x++) {
-            v0 += red[(x * S::CHUNK + tile * 4 + e) * 32 + lane];
-            v1 += red[(x * S::CHUNK + tile * 4 + e + 2) * 32 + lane];
+            const float4 u = red[(x * S::CHUNK + warp) * 32 + lane];
+            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
           }
-          if (whole) {
-            put(ch * CI + k, nt, e, v0, v1);
-          } else {
-            const int at = (ch * (S::CHUNK / 2) + pr) * 64 + lane * 2;
-            __stcg(reinterpret_cast<float2 *>(part + at), make_float2(v0, v1));
-          }
+          if (last) put(at / NT, at % NT, v);
+          else __stcg(reinterpret_cast<float4 *>(part) + at * 32 + lane, v);
         }
+        sync();
       }
-      sync();
-    }
-    if (!whole) {
-      if (tid < NC) {
-        __stcg(part + S::ACC * 32 + tid, um[tid]);
-        __stcg(part + S::ACC * 32 + NC + tid, ul[tid]);
+      if (last) break;
+      // a part: the last of the unit's CTAs to come joins all of them, a warp every fourth part
+      if (tid < COLS) {
+        __stcg(part + S::ACC * 128 + tid, um[tid]);
+        __stcg(part + S::ACC * 128 + COLS + tid, ul[tid]);
       }
       // the CTAs that share the unit, by the places of its first and last tile
       const int64_t u0 = line.at + kPad, u1 = u0 + line.tiles - 1;
@@ -706,57 +739,59 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
       sync();
       if (tid == 0) arrived = atomicAdd(&a.counters[c0], 1u);
       sync();
-      if (arrived == (uint32_t)(c1 - c0)) {
-        __threadfence();
-        if (tid == 0) a.counters[c0] = 0;
-        const auto part_of = [&](int x) { return a.parts + ((int64_t)x * 2 + (x == c0)) * S::PART; };
-        // a column's maximum and sum over the parts, a warp to a column; its weights for kBatch parts at a time
-        constexpr int kBatch = S::RED / 4 / NC;
-        for (int col = warp; col < NC; col += NW) {
-          float top = -INFINITY, sum = 0.0f;
-          for (int x = c0 + lane; x <= c1; x += 32) {
-            const float *p = part_of(x) + S::ACC * 32 + col;
-            const float pm = __ldcg(p), pl = __ldcg(p + NC);
-            if (pm == -INFINITY) continue;
-            const float v = fmaxf(top, pm);
-            sum = sum * ex2(top - v) + pl * ex2(pm - v);
-            top = v;
-          }
-          const float all = warp_max(top);
-          sum = warp_sum(top == -INFINITY ? 0.0f : sum * ex2(top - all));
-          if (lane == 0) um[col] = all, ul[col] = sum;
+      if (arrived != (uint32_t)(c1 - c0)) break;
+      __threadfence();
+      if (tid == 0) a.counters[c0] = 0;
+      const auto part_of = [&](int x) { return a.parts + ((int64_t)x * 2 + (x == c0)) * S::PART; };
+      // a column's maximum and sum over the parts, a warp to a column; its weights for kBatch parts at a time
+      constexpr int kBatch = S::RED / 4 / COLS;
+      float *weights = reinterpret_cast<float *>(red);
+      for (int col = warp; col < COLS; col += NW) {
+        float top = -INFINITY, sum = 0.0f;
+        for (int x = c0 + lane; x <= c1; x += 32) {
+          const float *p = part_of(x) + S::ACC * 128 + col;
+          const float pm = __ldcg(p), pl = __ldcg(p + COLS);
+          if (pm == -INFINITY) continue;
+          const float v = fmaxf(top, pm);
+          sum = sum * ex2(top - v) + pl * ex2(pm - v);
+          top = v;
         }
-        constexpr int PP = (S::ACC / 2 + NW - 1) / NW;   // pairs of accumulators of a warp
-        float2 v[PP];
+        const float all = warp_max(top);
+        sum = warp_sum(top == -INFINITY ? 0.0f : sum * ex2(top - all));
+        if (lane == 0) um[col] = all, ul[col] = sum;
+      }
 #pragma unroll
-        for (int y = 0; y < PP; y++) v[y] = make_float2(0.0f, 0.0f);
-        for (int x0 = c0; x0 <= c1; x0 += kBatch) {
-          const int n = min(kBatch, c1 - x0 + 1);
-          sync();
-          for (int i = tid; i < n * NC; i += NW * 32) {
-            const float pm = __ldcg(part_of(x0 + i / NC) + S::ACC * 32 + i % NC);
-            red[i] = pm == -INFINITY ? 0.0f : ex2(pm - um[i % NC]);
-          }
-          sync();
-#pragma unroll 4
-          for (int x = 0; x < n; x++) {
-            const float *p = part_of(x0 + x) + lane * 2;
+      for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int y = 0; y < PP; y++) {
-              const int pr = y * NW + warp, col = (pr >> 1) % NT * 8 + 2 * cq + (pr & 1);
-              if (pr < S::ACC / 2) {
-                const float2 u = __ldcg(reinterpret_cast<const float2 *>(p + pr * 64));
-                const float f = red[x * NC + col];
-                if (f != 0.0f) v[y].x += u.x * f, v[y].y += u.y * f;
-              }
+        for (int e = 0; e < 2; e++) {
+          f[nt][e] = 1.0f;
+#pragma unroll
+          for (int gr = 0; gr < GR; gr++) z[gr][nt][e] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < GR * 4; i++) o[i][nt][e] = o[i][nt][2 + e] = 0.0f;
+        }
+      for (int x0 = c0; x0 <= c1; x0 += kBatch) {
+        const int n = min(kBatch, c1 - x0 + 1);
+        sync();
+        for (int i = tid; i < n * COLS; i += NW * 32) {
+          const float pm = __ldcg(part_of(x0 + i / COLS) + S::ACC * 128 + i % COLS);
+          weights[i] = pm == -INFINITY ? 0.0f : ex2(pm - um[i % COLS]);
+        }
+        sync();
+        if (used)
+          for (int x = warp; x < n; x += NW) {
+            const float4 *p = reinterpret_cast<const float4 *>(part_of(x0 + x)) + lane;
+            float4 u[S::ACC];
+#pragma unroll
+            for (int y = 0; y < S::ACC; y++) u[y] = __ldcg(p + y * 32);
+#pragma unroll
+            for (int y = 0; y < S::ACC; y++) {
+              const int i = y / NT, nt = y % NT;
+              const float f0 = weights[x * COLS + nt * 8 + 2 * cq], f1 = weights[x * COLS + nt * 8 + 2 * cq + 1];
+              if (f0 != 0.0f) o[i][nt][0] += u[y].x * f0, o[i][nt][2] += u[y].z * f0;
+              if (f1 != 0.0f) o[i][nt][1] += u[y].y * f1, o[i][nt][3] += u[y].w * f1;
             }
           }
-        }
-#pragma unroll
-        for (int y = 0; y < PP; y++) {
-          const int pr = y * NW + warp;
-          if (pr < S::ACC / 2) put((pr >> 1) / NT, (pr >> 1) % NT, pr & 1, v[y].x, v[y].y);
-        }
       }
       sync();
     }
@@ -767,14 +802,14 @@ __global__ void __launch_bounds__(Shape<HD, BITS, NT>::NW * 32 + 32, Shape<HD, B
       mbar_wait(&full[i % STAGES], (i / STAGES) & 1, &g_paged_status, false);
 }
 
-template <int HD, int BITS, int NT>
+template <int HD, int BITS, int COLS>
 int launch(const PagedView &v, AttnParams &p, const Sm100PagedAttnArgs *a, cudaStream_t st) {
-  using S = Shape<HD, BITS, NT>;
+  using S = Shape<HD, BITS, COLS>;
   static int grid[64];   // CTAs that one device holds at once, by ordinal
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess || dev >= 64) return sm100_set_error(SM100_ERR_CUDA, "paged_attention: device %d: %s", dev, cudaGetErrorString(e));
-  const auto kernel = paged_attn_kernel<HD, BITS, NT>;
+  const auto kernel = paged_attn_kernel<HD, BITS, COLS>;
   if (!grid[dev]) {
     int sms = 0, per = 0;
     if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM)) != cudaSuccess ||
@@ -791,12 +826,22 @@ int launch(const PagedView &v, AttnParams &p, const Sm100PagedAttnArgs *a, cudaS
   return launch_status("paged_attention");
 }
 
+// Query columns of a unit: the fewest that hold a sequence's rows and heads of a group, at most 16 (8 at 256 dimensions, where
+// the accumulators of 16 would not fit the registers).
+int columns_of(int head_dim, int bits, int64_t cols) {
+  return cols > 8 && head_dim <= 128 ? 16 : cols > 4 || bits == 16 ? 8 : 4;
+}
+
 template <int HD, int BITS>
 int launch_columns(const PagedView &v, AttnParams &p, const Sm100PagedAttnArgs *a, cudaStream_t st) {
+  const int cols = columns_of(HD, BITS, (int64_t)a->max_rows * p.group);
   if constexpr (HD <= 128) {
-    if ((int64_t)a->max_rows * p.group > 8) return launch<HD, BITS, 2>(v, p, a, st);
+    if (cols == 16) return launch<HD, BITS, 16>(v, p, a, st);
   }
-  return launch<HD, BITS, 1>(v, p, a, st);
+  if constexpr (BITS == 4) {
+    if (cols == 4) return launch<HD, BITS, 4>(v, p, a, st);
+  }
+  return launch<HD, BITS, 8>(v, p, a, st);
 }
 
 }  // namespace
@@ -804,8 +849,8 @@ int launch_columns(const PagedView &v, AttnParams &p, const Sm100PagedAttnArgs *
 extern "C" uint64_t sm100_paged_attention_ws_bytes(const Sm100PagedCache *c, int32_t heads, int32_t max_rows) {
   PagedView v;
   if (sm100_paged_view(c, "paged_attention_ws_bytes", &v) || heads < 1 || heads % c->kv_heads || max_rows < 1) return 0;
-  const uint64_t cols = (uint64_t)max_rows * (heads / c->kv_heads) > 8 && c->head_dim <= 128 ? 16 : 8;
-  return kMaxPieces * 4 + (uint64_t)kMaxPieces * 2 * (cols * c->head_dim + 2 * cols) * 4;
+  const uint64_t cols = columns_of(c->head_dim, c->bits, (int64_t)max_rows * (heads / c->kv_heads));
+  return kMaxPieces * 4 + (uint64_t)kMaxPieces * 2 * ((cols < 8 ? 8 : cols) * c->head_dim + 2 * cols) * 4;
 }
 
 extern "C" int sm100_paged_attention(const Sm100PagedCache *c, const Sm100PagedAttnArgs *a, void *stream) {
