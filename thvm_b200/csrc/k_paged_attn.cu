@@ -245,9 +245,9 @@ struct Line {
 
 // Waits for a free stage: the copies' warp has time, and a busy wait would take issue slots from the products.
 __device__ __forceinline__ bool wait_free(uint64_t *bar, uint32_t parity) {
-  for (uint32_t i = 0; i < (1u << 22); i++) {
+  for (uint32_t i = 0; i < (1u << 20); i++) {
     if (mbar_try_wait(bar, parity)) return true;
-    __nanosleep(64);
+    __nanosleep(400);
   }
   atomicOr(&g_paged_status, SM100_DECODE_ERR_STALL);
   return false;
