@@ -778,18 +778,30 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
           weights[i] = pm == -INFINITY ? 0.0f : ex2(pm - um[i % COLS]);
         }
         sync();
-        if (used)
-          for (int x = warp; x < n; x += NW) {
-            const float4 *p = reinterpret_cast<const float4 *>(part_of(x0 + x)) + lane;
-            float4 u[S::ACC];
+        // a warp's parts, UN of them under way at a time; with 4 columns the idle half of the lanes takes every other one
+        // (the joining adds its columns to the first half's)
+        constexpr int UN = S::ACC <= 8 ? 2 : 1, SIDES = DUAL ? 2 : 1;
+        const int side = DUAL ? cq >> 1 : 0;
+        if (DUAL || used)
+          for (int x = warp + NW * side; x < n; x += NW * SIDES * UN) {
+            float4 u[UN][S::ACC];
 #pragma unroll
-            for (int y = 0; y < S::ACC; y++) u[y] = __ldcg(p + y * 32);
+            for (int k = 0; k < UN; k++) {
+              const int y = x + k * NW * SIDES;
+              const float4 *p = reinterpret_cast<const float4 *>(part_of(x0 + y)) + (DUAL ? lane & ~2 : lane);
 #pragma unroll
-            for (int y = 0; y < S::ACC; y++) {
-              const int i = y / NT, nt = y % NT;
-              const float f0 = weights[x * COLS + nt * 8 + 2 * cq], f1 = weights[x * COLS + nt * 8 + 2 * cq + 1];
-              if (f0 != 0.0f) o[i][nt][0] += u[y].x * f0, o[i][nt][2] += u[y].z * f0;
-              if (f1 != 0.0f) o[i][nt][1] += u[y].y * f1, o[i][nt][3] += u[y].w * f1;
+              for (int i = 0; i < S::ACC; i++) u[k][i] = y < n ? __ldcg(p + i * 32) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int k = 0; k < UN; k++) {
+              const int y = min(x + k * NW * SIDES, n - 1);
+#pragma unroll
+              for (int j = 0; j < S::ACC; j++) {
+                const int i = j / NT, nt = j % NT, col = column(nt * 8 + 2 * cq);
+                const float f0 = weights[y * COLS + col], f1 = weights[y * COLS + col + 1];
+                if (f0 != 0.0f) o[i][nt][0] += u[k][j].x * f0, o[i][nt][2] += u[k][j].z * f0;
+                if (f1 != 0.0f) o[i][nt][1] += u[k][j].y * f1, o[i][nt][3] += u[k][j].w * f1;
+              }
             }
           }
       }
