@@ -343,6 +343,46 @@ def test_attention_leaves_out_pages_outside_the_pool():
         assert c.status() == L.DECODE_ERR_ARG
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("hd,H,kv", [(64, 4, 2), (128, 8, 1), (256, 4, 2)])
+def test_later_tokens_that_are_not_finite_stay_out_of_earlier_rows(bits, hd, H, kv):
+    """Five new rows a sequence; the keys and values of the last two tokens hold NaN and infinities: the rows before
+    them are as without, the rows that see them are not finite."""
+    import torch
+    rng = np.random.default_rng(hd + bits)
+    lens, rows = [70, 16, 5], [5, 5, 5]
+    c = _cache(lens, kv, hd, 16, bits, rng)
+    _fill(c, lens, rng)
+    T = sum(rows)
+    q = torch.from_numpy(rng.standard_normal((T, H, hd)).astype(np.float32)).cuda().bfloat16()
+    want, size = _attend_want(c, q, lens, rows, hd ** -0.5)
+    bad = torch.from_numpy(rng.standard_normal((6, 3 * kv * hd)).astype(np.float32)).cuda()
+    bad[0::2] = float("nan")
+    bad[1::2, ::3] = float("inf")
+    pos = torch.tensor([x for n in lens for x in (n - 2, n - 1)], dtype=torch.int32).cuda()
+    c.append(bad, pos, torch.tensor([0, 0, 1, 1, 2, 2], dtype=torch.int32).cuda(), kv)
+    got = c.attend(q, torch.tensor(lens, dtype=torch.int32).cuda(),
+                   q_off=torch.tensor([0, 5, 10, 15], dtype=torch.int32).cuda(), max_rows=5)
+    early = torch.tensor([5 * s + r for s in range(3) for r in range(3)]).cuda()
+    _check_attention(got[early], want[early], size[early])
+    late = torch.tensor([5 * s + r for s in range(3) for r in (3, 4)]).cuda()
+    assert bool(torch.isnan(got[late]).any(-1).all())
+
+
+def test_attention_repeats_to_the_bit():
+    """Units cut between CTAs are joined in one order, whichever CTA comes last."""
+    import torch
+    rng = np.random.default_rng(13)
+    for bits, lens in ((4, [9000, 3]), (16, [3000, 700, 1])):
+        c = _cache(lens, 2, 128, 64, bits, rng)
+        _fill(c, lens, rng)
+        q = torch.from_numpy(rng.standard_normal((len(lens), 8, 128)).astype(np.float32)).cuda().bfloat16()
+        kv_len = torch.tensor(lens, dtype=torch.int32).cuda()
+        first = c.attend(q, kv_len)
+        for _ in range(30):
+            assert torch.equal(c.attend(q, kv_len), first)
+
+
 def test_attention_offsets_past_two_gigabytes():
     """A pool of 5 GB whose used pages lie at its far end."""
     import torch
@@ -431,6 +471,8 @@ def test_refusals():
         c.attend(torch.zeros(2, 3, 64, dtype=torch.bfloat16, device="cuda"), i(1, 1))   # 3 heads on 2
     with pytest.raises(L.Sm100Error):
         c.attend(q[:1], i(1, 1))        # one row for two sequences, no offsets
+    with pytest.raises(L.Sm100Error):
+        c.attend(q, i(1, 1), scale=-0.5)
     assert c.attend(q[:0], i(0, 0), q_off=i(0, 0, 0)).shape == (0, 4, 64)
     small = L.Sm100PagedAttnArgs(q.data_ptr(), c.table.data_ptr(), None, q.data_ptr(), q.data_ptr(), 0, 0, 2, 4, 1, 1.0)
     assert L.lib().sm100_paged_attention(c._desc, ctypes.byref(small), None) == L.ERR_ARG

@@ -165,6 +165,25 @@ def test_rows_with_nothing_nan_and_infinities():
     assert _run(x, torch.tensor([[1, 1, 1e-30, 1e-20]]).cuda(), k=3)[0].tolist() == [2]
 
 
+def test_many_rows_on_every_cluster_size_repeat_to_the_bit():
+    """The same rows in batches of every launch shape, and again: ids and log-probabilities do not move."""
+    import torch
+    g = torch.Generator("cuda")
+    g.manual_seed(9)
+    V = 40001
+    x = 2 * torch.randn(200, V, device="cuda", generator=g)
+    x = (x * 8).round() / 8   # many equal logits
+    noise = torch.empty(200, V, device="cuda").exponential_(generator=g)
+    f = dict(T=0.9, p=0.95)
+    tok, logp = _run(x, noise, **f)
+    for _ in range(3):
+        again = _run(x, noise, **f)
+        assert torch.equal(again[0], tok) and torch.equal(again[1], logp)
+    for n in (1, 20, 100):
+        t, lp = _run(x[:n], noise[:n], **f)
+        assert torch.equal(t, tok[:n]) and float((lp - logp[:n]).abs().max()) <= 1e-5
+
+
 def test_probabilities_of_the_draw():
     """20000 draws over 12 ids with top-p: frequencies within 5 standard deviations of the kept ids' probabilities,
     none of the others."""

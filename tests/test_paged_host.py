@@ -79,7 +79,8 @@ def test_attention_refusals():
     c = _cache()
     for bad in (dict(q=None), dict(kv_len=None), dict(out=None), dict(ws=None), dict(T=-1), dict(heads=3),
                 dict(max_rows=0), dict(q_off=None, T=1), dict(q_off=None, max_rows=2), dict(q=P + 8), dict(out=P + 8),
-                dict(ws=P + 8), dict(ld_q=100), dict(ld_q=260), dict(ws_bytes=0)):
+                dict(ws=P + 8), dict(ld_q=100), dict(ld_q=260), dict(ws_bytes=0), dict(scale=-1.0), dict(scale=float("nan")),
+                dict(scale=float("inf"))):
         assert _attend(c, **bad) == L.ERR_ARG, bad
     assert _attend(c, T=0) == L.OK
     assert L.lib().sm100_paged_attention_ws_bytes(ctypes.byref(c), 4, 1) > 0

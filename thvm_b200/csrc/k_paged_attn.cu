@@ -324,8 +324,8 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
       if (!ok_ring || line.at + kPad + line.tiles >= w1) break;
       line.next();
     }
-    if (lane == 0 && me == 0) {   // lengths past the table were cut
-      for (int s = 0; s < c.n_seq; s++)
+    if (me == 0) {   // lengths past the table were cut
+      for (int s = lane; s < c.n_seq; s += 32)
         if (a.kv_len[s] > c.max_pages * c.page) atomicOr(&g_paged_status, SM100_DECODE_ERR_ARG);
     }
     return;
@@ -882,6 +882,8 @@ extern "C" int sm100_paged_attention(const Sm100PagedCache *c, const Sm100PagedA
   if (a->ws_bytes < need)
     return sm100_set_error(SM100_ERR_ARG, "paged_attention: %llu bytes of scratch, %llu needed",
                            (unsigned long long)a->ws_bytes, (unsigned long long)need);
+  if (!(a->scale >= 0.0f && a->scale <= 3e38f))
+    return sm100_set_error(SM100_ERR_ARG, "paged_attention: scale %g (0 or more, finite)", (double)a->scale);
   if ((int64_t)a->T * a->heads / c->kv_heads > INT32_MAX)
     return sm100_set_error(SM100_ERR_ARG, "paged_attention: %d rows in one call", a->T);
   AttnParams p{static_cast<const __nv_bfloat16 *>(a->q), a->kv_len, a->q_off, static_cast<__nv_bfloat16 *>(a->out),
