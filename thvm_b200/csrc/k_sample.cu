@@ -44,7 +44,7 @@ using namespace sm100;
 namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = 4096, kCap = 2048;
+constexpr int kBins = 4096, kCap = 2048, kMost = 8;   // kMost: CTAs of a row
 constexpr float kPerNat = 128.0f;
 
 struct SampleParams {
@@ -146,14 +146,16 @@ struct alignas(16) Shared {
   uint64_t few[32], pick_over;
   uint32_t pick_n, n_few;
   uint64_t red[kWarps], red2[kWarps];
-  // read by the other CTAs of the cluster
-  uint64_t top, row, near, above, best, kept;   // largest place; weight of all ids, of those in the bins; measure above them;
-                                               // winner; kept weight
-  uint32_t n_list, ids;                   // gathered places; ids in this CTA's slice of bins
-  float heavy;                            // and their estimated weight
-  // of CTA 0, written by whoever finds it
-  Crossing cross[kGoals + 1];   // kLast: the last bin that matters
-  uint64_t cut, sum, over;
+  uint32_t n_list;                 // gathered places
+  Crossing cross[kGoals + 1];      // kLast: the last bin that matters
+  // what each CTA of the cluster has pushed here: a push and a barrier are one hop, a read after the barrier another
+  struct {
+    uint64_t top, row, near, above, best, kept;   // largest place; weight of all ids, of those in the bins; measure above the
+                                                  // list's bins; winner there and kept weight
+    uint32_t ids, n_list;                         // ids in its slice of bins; places on its list
+    float heavy;                                  // the slice's estimated weight
+  } from[kMost];
+  uint64_t cut, sum, over;         // from CTA 0
   uint32_t done, missed;
 };
 
@@ -281,6 +283,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const int rank = C > 1 ? (int)cluster.block_rank() : 0, tid = threadIdx.x;
   const int b = blockIdx.x / C;
   pdl_trigger();
+  if constexpr (C > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   for (int i = tid; i < kBins; i += kThreads) sh.hist[i] = 0;
   pdl_wait();
   const int begin = min(rank * a.chunk, a.V), n = min(a.V - begin, a.chunk);
@@ -334,10 +337,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       if (imax + e < n && raw(imax + e) == lmax) top = place(clean(lmax), begin + imax + e);
   }
   top = block_max64(top, sh.red);
-  if (tid == 0) sh.top = top, sh.n_list = 0;
+  if (tid == 0) sh.n_list = 0;
+  if (tid <= kGoals) sh.cross[tid].bin = -1;
+  if constexpr (C > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");   // every CTA has begun
+  // the shared memory of CTA tid, for the threads that push a value to every CTA
+  Shared *to = tid < C ? (C > 1 ? cluster.map_shared_rank(&sh, tid) : &sh) : nullptr;
+  if (to) to->from[rank].top = top;
   sync();
-  // a value of every CTA of the cluster by the lanes of each warp: one round trip
-  const Shared *peer = C > 1 ? cluster.map_shared_rank(&sh, (tid & 31) % C) : &sh;
+  const auto *peer = &sh.from[(tid & 31) % C];   // the lanes of each warp take what every CTA has pushed
   const auto cluster_sum = [&](uint64_t v) {
     v = (tid & 31) < C ? v : 0;
 #pragma unroll
@@ -356,7 +363,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       a.tok[b] = top == 0 ? -1 : id_of(top);
       if (a.logp) a.logp[b] = top == 0 ? -INFINITY : 0.0f;
     }
-    sync();   // the others may still read this CTA's first place
     return;
   }
   Scale sc;
@@ -364,7 +370,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const bool wild = sc.lmax == FLT_MAX;   // there may be +inf among the logits
   const float min_p = a.min_p ? a.min_p[b] : 0.0f, p = a.top_p ? a.top_p[b] : 1.0f;
   const int k = a.top_k ? a.top_k[b] : 0;
-  Shared *first = C > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
   // a vector as floats; NaN stays (it fails every comparison below)
   const auto floats = [&](const uint4 &v, float x[E]) {
     const In *y = reinterpret_cast<const In *>(&v);
@@ -390,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       else c++;
     });
     const uint64_t s = block_sum64(weigh ? fixed(w) : c, sh.red);
-    if (tid == 0) sh.row = s;
+    if (to) to->from[rank].row = s;
     sync();
     const uint64_t all = cluster_sum(peer->row);
     sync();
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     }
     if (by_weight) {
       const uint64_t s = block_sum64(fixed(w), sh.red), f = block_sum64(fixed(w_near), sh.red2);
-      if (tid == 0) sh.row = s, sh.near = f;
+      if (to) to->from[rank].row = s, to->from[rank].near = f;
     }
     sync();
     {
@@ -471,8 +476,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     for (int i = 0; i < kB; i++) ids += cnt[i], heavy += cnt[i] * __expf(-(float)(bin0 + i) / kPerNat);
     c_before = block_before(ids, reinterpret_cast<uint32_t *>(sh.red), &ids);
     w_before = block_before(heavy, reinterpret_cast<float *>(sh.red2), &heavy);
-    if (tid == 0) sh.ids = ids, sh.heavy = heavy;
-    if (rank == 0 && tid < kGoals) sh.cross[tid].bin = -1;
+    if (to) to->from[rank].ids = ids, to->from[rank].heavy = heavy;
     sync();
     const uint32_t c = (tid & 31) < C ? peer->ids : 0;
     const float h = (tid & 31) < C ? peer->heavy : 0.0f;
@@ -507,18 +511,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
           const float goals[kGoals] = {goal * (1.0f - 0.0045f * spread), goal * (1.0f + 0.0045f * spread),
                                        guess * (1.0f - 0.001f * spread), guess * (1.0f + 0.001f * spread),
                                        guess * (1.0f - 0.0002f * spread), guess * (1.0f + 0.0002f * spread), guess};
+          const auto tell = [&](int g, const Crossing &x) {
+            for (int r = 0; r < C; r++) (C > 1 ? cluster.map_shared_rank(&sh, r) : &sh)->cross[g] = x;
+          };
           uint32_t cc = c_before;
           float ww = w_before;
 #pragma unroll
           for (int i = 0; i < kB; i++) {
-            if (bin0 + i == last_bin) first->cross[kLast] = Crossing{last_bin, cc, cc + cnt[i], ww};
+            if (bin0 + i == last_bin) tell(kLast, Crossing{last_bin, cc, cc + cnt[i], ww});
             if (cnt[i] == 0 || bin0 + i > last_bin) continue;
             const uint32_t c1 = cc + cnt[i];
             const float w1 = ww + cnt[i] * __expf(-(float)(bin0 + i) / kPerNat);
 #pragma unroll
             for (int g = 0; g < kGoals; g++) {
               const float was = weigh ? ww : (float)cc, now = weigh ? w1 : (float)c1;
-              if (now >= goals[g] && (was < goals[g] || cc == 0)) first->cross[g] = Crossing{bin0 + i, cc, c1, ww};
+              if (now >= goals[g] && (was < goals[g] || cc == 0)) tell(g, Crossing{bin0 + i, cc, c1, ww});
             }
             cc = c1, ww = w1;
           }
@@ -528,9 +535,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         bool fits = false;
 #pragma unroll
         for (int g = 0; g < 4; g++) {
-          Crossing x = first->cross[g < 3 ? 2 * g : kGuess], y = first->cross[g < 3 ? 2 * g + 1 : kGuess];
-          if (x.bin < 0) x = first->cross[kLast];   // reached nowhere
-          if (y.bin < 0) y = first->cross[kLast];
+          Crossing x = sh.cross[g < 3 ? 2 * g : kGuess], y = sh.cross[g < 3 ? 2 * g + 1 : kGuess];
+          if (x.bin < 0) x = sh.cross[kLast];   // reached nowhere
+          if (y.bin < 0) y = sh.cross[kLast];
           if (g == 0 && attempt) continue;   // the guess knows more by now
           if (fits) continue;
           if (y.upto <= kCap) fits = true, lo = 0, before = 0.0f, hi = y.bin;
@@ -604,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         }
       }
       const uint64_t measured = whole ? 0 : block_sum64(weigh ? fixed(over) : n_over, sh.red);
-      if (tid == 0) sh.above = measured;
+      if (to) to->from[rank].above = measured;
       if (racing) {
         const uint64_t m = block_max64(best > -INFINITY ? place(clean(best), 0) : 0, sh.red2);
         const float from = logit_of(m) - 0.02f;
@@ -624,8 +631,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         }
         won = block_max64(won, sh.red);
         const uint64_t sum = block_sum64(fixed(kept), sh.red2);
-        if (tid == 0) sh.best = won, sh.kept = sum;
+        if (to) to->from[rank].best = won, to->from[rank].kept = sum;
       }
+      __syncthreads();
+      if (to) to->from[rank].n_list = sh.n_list;
       sync();
       if (rank == 0) {
         // the other CTAs' places behind this one's
@@ -657,12 +666,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             end = select(sh, m, end, 0, (double)p * (double)s, true, weight_of, &upto, &all);
         }
         const bool finish = in && (whole || final_round);
-        if (tid == 0) {
-          sh.missed = !in;
-          sh.cut = end;
-          sh.sum = s;
-          sh.over = above;
-          sh.done = finish;
+        if (to) {
+          to->missed = !in;
+          to->cut = end;
+          to->sum = s;
+          to->over = above;
+          to->done = finish;
         }
         if (finish) {   // the race over the list, and the winners above it
           uint64_t best1 = 0, kept1 = 0;
@@ -689,12 +698,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         }
       }
       sync();
-      const bool done = first->done, missed = first->missed;
-      const uint64_t new_cut = first->cut, sum = first->sum, exact_over = first->over;
+      if (sh.done) return;   // nothing reaches into another CTA past here
+      const bool missed = sh.missed;
+      const uint64_t new_cut = sh.cut, sum = sh.sum, exact_over = sh.over;
       if (tid == 0) sh.n_list = 0;
-      sync();   // CTA 0's words are free again, and its shared memory is not needed by others past here
-      if (done) return;
-      if (rank == 0 && tid < kGoals) sh.cross[tid].bin = -1;
+      if (tid <= kGoals) sh.cross[tid].bin = -1;
       sync();
       if (!missed) {
         bisect = false;
@@ -730,7 +738,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   });
   const uint64_t all = block_sum64(fixed(kept), sh.red);
   won = block_max64(won, sh.red2);
-  if (tid == 0) sh.kept = all, sh.best = won;
+  if (to) to->from[rank].kept = all, to->from[rank].best = won;
   sync();
   if (rank == 0 && tid < 32) {
     const uint64_t w = cluster_max(peer->best), sum = cluster_sum(peer->kept);
@@ -740,7 +748,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       if (a.logp) a.logp[b] = sc.d(clean(to_float(static_cast<const In *>(a.logits)[b * a.ld + id]))) - logf((float)sum * 0x1p-40f);
     }
   }
-  sync();
 }
 
 constexpr int kHeld = 64 * 1024;   // bytes of a row that a CTA holds: two CTAs an SM
