@@ -358,7 +358,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     return __shfl_sync(0xffffffffu, v, 0);
   };
   top = cluster_max(peer->top);
-  if (top == 0 || !(T > 0.0f)) {
+  const float min_p = a.min_p ? a.min_p[b] : 0.0f;
+  if (top == 0 || !(T > 0.0f) || !(min_p <= 1.0f)) {   // nothing, or the first id alone
     if (rank == 0 && tid == 0) {
       a.tok[b] = top == 0 ? -1 : id_of(top);
       if (a.logp) a.logp[b] = top == 0 ? -INFINITY : 0.0f;
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   Scale sc;
   sc.set(logit_of(top), T);
   const bool wild = sc.lmax == FLT_MAX;   // there may be +inf among the logits
-  const float min_p = a.min_p ? a.min_p[b] : 0.0f, p = a.top_p ? a.top_p[b] : 1.0f;
+  const float p = a.top_p ? a.top_p[b] : 1.0f;
   const int k = a.top_k ? a.top_k[b] : 0;
   // a vector as floats; NaN stays (it fails every comparison below)
   const auto floats = [&](const uint4 &v, float x[E]) {
@@ -402,11 +403,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     return all;
   };
   const float *noise = a.noise + b * a.ld_noise + begin;
-  const int itop = id_of(top) - begin;   // in the CTA's own count
   const float inv = fminf(1.0f / T, 1e38f);
   const auto score = [&](float l, int i) { return sc.d(l) - logf(__ldg(noise + i)); };
   const auto fast_score = [&](float l, float e) { return (l - sc.lmax) * inv - __logf(e); };
-  const auto passes = [&](float l, int i) { return sc.weight(l) >= min_p || i == itop; };
+  const auto passes = [&](float l) { return sc.weight(l) >= min_p; };   // the first id's is 1
 
   uint64_t cut = 1, total = 0, near = 0;   // kept: place >= cut; what a top-p is a part of; of that what the bins hold
   bool past = false;
@@ -540,57 +540,56 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
           if (y.bin < 0) y = sh.cross[kLast];
           if (g == 0 && attempt) continue;   // the guess knows more by now
           if (fits) continue;
-          if (y.upto <= kCap) fits = true, lo = 0, before = 0.0f, hi = y.bin;
-          else if (y.upto - x.before <= kCap) fits = true, lo = x.bin, before = x.weight_before, hi = y.bin;
+          if (y.upto <= kCap - 64) fits = true, lo = 0, before = 0.0f, hi = y.bin;
+          else if (y.upto - x.before <= kCap - 64) fits = true, lo = x.bin, before = x.weight_before, hi = y.bin;
         }
         if (!fits) break;
       }
       // ---- the pass: ids above the bins are measured and, in the last round, race; those in the bins go on the list.  Of its
       // race a thread keeps the best two scores by fast math; what is within its error of the CTA's best is scored exactly
-      const float f_lo = filtered ? 12582912.0f + lo : INFINITY;
-      const float f_hi = filtered ? hi == kBins - 1 ? INFINITY : 12582912.0f + hi : -INFINITY;
+      // By logit: above x_lo is above the bins, down to x_hi on the list (a hundredth of a bin and some roundings more than the
+      // bins hold; what the pass sums and gathers is what counts)
       const bool whole = filtered && lo == 0, racing = final_round && !whole;   // whole: the list holds all that is kept
+      const float slack = 1e-6f * fabsf(sc.lmax);
+      const float x_lo = !filtered ? l_far : whole ? INFINITY : sc.lmax - (lo - 0.51f) / sc.per * 0.999999f + slack;
+      const float x_hi = !filtered ? INFINITY : hi == kBins - 1 ? -FLT_MAX : sc.lmax - (hi + 0.51f) / sc.per * 1.000001f - slack;
+      const float x_any = fminf(x_lo, x_hi);   // below it a vector has nothing for this pass: most of a peaked row
       float over = 0.0f, kept = 0.0f, best = -INFINITY, second = -INFINITY;
       uint32_t n_over = 0;
       int best_i = -1;
-      // below every bin that matters: most vectors of a peaked row
-      const float l_skip = !filtered ? l_far : hi < kBins - 1 ? sc.lmax - (hi + 1) / sc.per * 1.00001f : -INFINITY;
 #pragma unroll 2
       for (int i = tid; i < nv; i += kThreads) {
         const uint4 v = vector(i);
-        if (!(largest(v, In()) >= l_skip)) continue;
+        const float most = largest(v, In());
+        if (!(most >= x_any)) continue;
         float x[E];
         floats(v, x);
-        uint32_t above = 0, in = 0;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-          const float bin = sc.bin_float(x[e]);
-          above |= bin < f_lo ? 1u << e : 0u;
-          in |= bin >= f_lo && bin <= f_hi ? 1u << e : 0u;
-        }
-        if (above && !whole) {
+        if (most > x_lo) {
           float e[E];
           if (racing) {
 #pragma unroll
             for (int q = 0; q < E; q += 4) {   // the random numbers of four ids where one of them is kept
               e[q] = e[q + 1] = e[q + 2] = e[q + 3] = 1.0f;
-              if (a.noise_vec && (above >> q & 15) && i * E + q + 4 <= n) {
-                const float4 v = __ldg(reinterpret_cast<const float4 *>(noise + i * E + q));
-                e[q] = v.x, e[q + 1] = v.y, e[q + 2] = v.z, e[q + 3] = v.w;
+              if (a.noise_vec && i * E + q + 4 <= n) {
+                if (fmaxf(fmaxf(x[q], x[q + 1]), fmaxf(x[q + 2], x[q + 3])) > x_lo) {
+                  const float4 r = __ldg(reinterpret_cast<const float4 *>(noise + i * E + q));
+                  e[q] = r.x, e[q + 1] = r.y, e[q + 2] = r.z, e[q + 3] = r.w;
+                }
               } else {
 #pragma unroll
                 for (int j = q; j < q + 4; j++)
-                  if (above >> j & 1) e[j] = __ldg(noise + i * E + j);
+                  if (x[j] > x_lo) e[j] = __ldg(noise + i * E + j);
               }
             }
           }
-          n_over += __popc(above);
 #pragma unroll
           for (int j = 0; j < E; j++) {
-            const float w = above >> j & 1 ? sc.weight(x[j]) : 0.0f;
+            const bool up = x[j] > x_lo;
+            const float w = up ? sc.weight(x[j]) : 0.0f;
             over += w;
+            if (!weigh) n_over += up;
             if (racing) {
-              const bool runs = (above >> j & 1) && (w >= min_p || i * E + j == itop);
+              const bool runs = up && w >= min_p;
               kept += runs ? w : 0.0f;
               const float f = runs ? fast_score(x[j], e[j]) : -INFINITY;
               second = fmaxf(second, fminf(f, best));
@@ -598,6 +597,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             }
           }
         }
+        uint32_t in = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++) in |= x[e] >= x_hi && x[e] <= x_lo ? 1u << e : 0u;
         while (in) {
           const int e = __ffs(in) - 1;
           in &= in - 1;
@@ -624,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
           for (int i = tid; i < nv; i += kThreads)
             for (int j = i * E; j < min((i + 1) * E, n); j++) {
               const float l = clean(raw(j));
-              if (sc.bin_float(l) < f_lo && passes(l, j) && fast_score(l, __ldg(noise + j)) >= from) exact(l, j);
+              if (l > x_lo && passes(l) && fast_score(l, __ldg(noise + j)) >= from) exact(l, j);
             }
         } else if (m != 0 && best >= from) {
           exact(clean(raw(best_i)), best_i);
@@ -679,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             for (uint32_t x = tid; x < m; x += kThreads) {
               const uint64_t pl = sh.list[x];
               const float l = logit_of(pl), w1 = sc.weight(l);
-              if (pl < end || (!(w1 >= min_p) && pl != top)) continue;
+              if (pl < end || !(w1 >= min_p)) continue;
               kept1 += fixed(w1);
               const float s1 = sc.d(l) - logf(__ldg(a.noise + b * a.ld_noise + id_of(pl)));
               if (s1 > -INFINITY) best1 = max64(best1, place(clean(s1), id_of(pl)));
@@ -707,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       if (!missed) {
         bisect = false;
         cut = new_cut;
-        if (!weigh && by_weight) total = sum + (lo > 0 ? measure_all(true, [&](float l, uint64_t) { return sc.bin(l) < lo; }) : 0);
+        if (!weigh && by_weight) total = sum + (lo > 0 ? measure_all(true, [&](float l, uint64_t) { return l > x_lo; }) : 0);
         break;
       }
       // what lies before bin lo is known now
@@ -731,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   uint64_t won = 0;
   each([&](float l, int i) {
     const uint64_t pl = place(l, begin + i);
-    if (pl < cut || !passes(l, i)) return;
+    if (pl < cut || !passes(l)) return;
     kept += sc.weight(l);
     const float s = score(l, i);
     if (s > -INFINITY) won = max64(won, place(clean(s), begin + i));
