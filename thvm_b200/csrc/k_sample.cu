@@ -308,6 +308,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     }
     return v;
   };
+  // this thread's vectors in rising order, the next two under way
+  const auto each_vector = [&](auto f) {
+    uint4 v = tid < nv ? vector(tid) : uint4(), next = tid + kThreads < nv ? vector(tid + kThreads) : uint4();
+#pragma unroll 1
+    for (int i = tid; i < nv; i += kThreads) {
+      const uint4 now = v;
+      v = next;
+      if (i + 2 * kThreads < nv) next = vector(i + 2 * kThreads);
+      f(now, i);
+    }
+  };
   const float T = a.temperature ? a.temperature[b] : 1.0f;
 
   // ---- the row into shared memory, and its first place
@@ -430,9 +441,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     if (!(by_count && by_weight) && min_p > 0.0f) x_far = fmaxf(x_far, logf(fminf(min_p, 1.0f)) - 1e-3f);
     l_far = fminf(sc.lmax + x_far * T, nextafterf(sc.lmax, -INFINITY));
     float w = 0.0f, w_near = 0.0f;
-#pragma unroll 2
-    for (int i = tid; i < nv; i += kThreads) {
-      const uint4 v = vector(i);
+    each_vector([&](const uint4 &v, int) {
       float x[E];
       floats(v, x);
       if (by_weight) {
@@ -446,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
           if (by_weight) w_near += x[e] > l_far ? sc.weight(x[e]) : 0.0f;
         }
       }
-    }
+    });
     if (by_weight) {
       const uint64_t s = block_sum64(fixed(w), sh.red), f = block_sum64(fixed(w_near), sh.red2);
       if (to) to->from[rank].row = s, to->from[rank].near = f;
@@ -557,11 +566,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       float over = 0.0f, kept = 0.0f, best = -INFINITY, second = -INFINITY;
       uint32_t n_over = 0;
       int best_i = -1;
-#pragma unroll 2
-      for (int i = tid; i < nv; i += kThreads) {
-        const uint4 v = vector(i);
+      each_vector([&](const uint4 &v, int i) {
         const float most = largest(v, In());
-        if (!(most >= x_any)) continue;
+        if (!(most >= x_any)) return;
         float x[E];
         floats(v, x);
         if (most > x_lo) {
@@ -611,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
           const uint32_t at = atomicAdd(&sh.n_list, 1u);
           if (at < kCap) sh.list[at] = pl;
         }
-      }
+      });
       const uint64_t measured = whole ? 0 : block_sum64(weigh ? fixed(over) : n_over, sh.red);
       if (to) to->from[rank].above = measured;
       if (racing) {
