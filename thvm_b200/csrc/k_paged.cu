@@ -16,9 +16,10 @@
 // keeps its rotation, page and norm weights in registers while it walks over the
 // heads, the next head's load under way.
 //
-// What bounds it: memory for many rows (16384 rows of 16 + 2 x 16 heads of 128,
-// bf16: 92 us, 4.5 TB/s of values read and written, next to ~130 instructions a
-// warp and step), the latency of seq -> page -> store for few.
+// What bounds it: for many rows memory and issue about alike (16384 rows of 16 +
+// 2 x 16 heads of 128, bf16: 91 us, 4.5 TB/s read and written, 150 instructions a
+// warp and step at 68 % of the issue slots; a second step's load under way
+// changes nothing), for few the latency of seq -> page -> store.
 #include "paged.cuh"
 
 using namespace sm100;
@@ -179,7 +180,8 @@ __global__ void __launch_bounds__(256, 4) paged_append_kernel(const PagedView c,
     next.get(x);
     if (h + HPW < n_heads) next = load_raw(src + (int64_t)(h + HPW) * HD);   // the next step's load under way
     const bool live = h < n_heads, is_q = h < a.heads, turns = h < a.heads + c.kv_heads;
-    if (a.g_q || a.g_k) {
+    const bool turning = h0 + i * HPW < a.heads + c.kv_heads;   // one of the step's heads is a query or a key
+    if (turning && (a.g_q || a.g_k)) {
       const float ss = sum_squares<HD>(x);
       const float *gp = is_q ? a.g_q : a.g_k;
       if (turns && gp) {
@@ -192,7 +194,7 @@ __global__ void __launch_bounds__(256, 4) paged_append_kernel(const PagedView c,
         for (int j = 0; j < 8; j++) x[j] = __fmul_rn(__fmul_rn(x[j], r), g[j]);
       }
     }
-    if (a.rot) {
+    if (turning && a.rot) {
       if (a.pairs) {
         if (in && turns) {
 #pragma unroll
@@ -202,7 +204,7 @@ __global__ void __launch_bounds__(256, 4) paged_append_kernel(const PagedView c,
             x[2 * j + 1] = __fadd_rn(__fmul_rn(w, cs[j]), __fmul_rn(u, sn[j]));
           }
         }
-      } else if (h0 + i * HPW < a.heads + c.kv_heads) {   // one of the step's heads turns
+      } else {
         float y[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) y[j] = __shfl_sync(0xffffffffu, x[j], partner);
