@@ -2,12 +2,12 @@
 // scale) v, query head h on key head h / (heads / kv_heads), row r of n on keys
 // 0 .. kv_len - n + r.
 //
-// What bounds it: every key and value is read once for up to 16 query columns
+// What bounds it: every key and value is read once for up to 8 query columns
 // (the heads of a group times the new rows), so a decode step is bound by
 // memory, and in 4 bits, where a token of 128 + 128 dimensions is 144 bytes, by
 // issue slots next to it (unpacking, about one instruction a value).
 //
-// Split.  The tiles (TS tokens) of all units (sequence, key head, 16 query
+// Split.  The tiles (TS tokens) of all units (sequence, key head, 8 query
 // columns) form one line that is cut into gridDim equal pieces, one per CTA, so
 // ragged lengths and one long sequence load every SM alike; the cut is found on
 // the device from kv_len, so a captured graph follows it.  A unit cut between
@@ -59,7 +59,10 @@ struct AttnParams {
 constexpr int kMaxPieces = 148 * 4;   // CTAs of a launch at most
 
 // COLS query columns a unit: 4 (4 bits only: the weights' low parts take the
-// other half of the 8 columns of a product), 8 or 16.
+// other half of the 8 columns of a product) or 8.  Two products a unit, 16
+// columns, unpack a token once for both but leave registers for two CTAs an SM
+// only: 8 x 4096 tokens in 4 bits with 32 columns a key head took 40 us, 34.5 in
+// units of 8.
 template <int HD, int BITS, int COLS>
 struct Shape {
   static constexpr int NW = 4;                                  // warps at the products
@@ -71,13 +74,12 @@ struct Shape {
   // a tile in shared memory: keys, their marks, values, their marks of all tokens
   static constexpr int V = TS * (ROW + MARKS), TILE = 2 * V;
   static constexpr bool DUAL = COLS == 4;
-  static constexpr int NT = COLS == 16 ? 2 : 1;                 // column tiles of 8
-  static constexpr int ACC = HD / 16 * NT;                      // accumulator tiles (4 floats) of a thread
+  static constexpr int ACC = HD / 16;                           // accumulator tiles (4 floats) of a thread
   static constexpr int CHUNK = 4;                               // of them joined at a time, one a warp
   static constexpr int PART = ACC * 128 + 2 * COLS;             // floats of a unit's part
   static constexpr int RED = NW * CHUNK * 512;
   // CTAs of an SM: what the registers leave (5 warps each: 128 registers at 3, 168 at 2)
-  static constexpr int CTAS = HD == 256 ? (BITS == 4 ? 2 : 1) : NT == 2 || (HD == 128 && BITS == 16) ? 2 : 3;
+  static constexpr int CTAS = HD == 256 ? (BITS == 4 ? 2 : 1) : HD == 128 && BITS == 16 ? 2 : 3;
   static constexpr int ROOM = 227 * 1024 / CTAS - RED - 3072;
   static constexpr int STAGES = ROOM / TILE > 8 ? 8 : ROOM / TILE;
   static constexpr int SMEM = STAGES * TILE + RED;
@@ -257,7 +259,7 @@ template <int HD, int BITS, int COLS>
 __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD, BITS, COLS>::CTAS)
     paged_attn_kernel(const __grid_constant__ PagedView c, const __grid_constant__ AttnParams a) {
   using S = Shape<HD, BITS, COLS>;
-  constexpr int NW = S::NW, KS = S::KS, TS = S::TS, NT = S::NT, STAGES = S::STAGES, GR = S::GR, ROW = S::ROW, MARKS = S::MARKS;
+  constexpr int NW = S::NW, KS = S::KS, TS = S::TS, STAGES = S::STAGES, GR = S::GR, ROW = S::ROW, MARKS = S::MARKS;
   constexpr bool DUAL = S::DUAL;
   extern __shared__ __align__(128) uint8_t smem[];
   float4 *red = reinterpret_cast<float4 *>(smem + STAGES * S::TILE);
@@ -344,69 +346,60 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
     if (t0 >= t1) break;   // the piece ends before the unit's first tile
     const int n_cols = min(COLS, line.rows * a.group - line.ct * COLS);
     // Q^T fragments: column g of each 8, this lane's dimensions
-    uint32_t qf[NT][HD / 8];
-    float qs[GR][NT][2];   // 4 bits: sum of a column's queries over a group (columns 2 cq, 2 cq + 1)
+    uint32_t qf[HD / 8];
+    float qs[GR][2];   // 4 bits: sum of a column's queries over a group (columns 2 cq, 2 cq + 1)
+    const int col = column(g), at = line.ct * COLS + col;
+    const __nv_bfloat16 *src = a.q + (int64_t)(line.first + at / a.group) * a.ld_q +
+                               (int64_t)(line.h * a.group + at % a.group) * HD;
+    uint4 v[HD / 32];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      const int col = column(nt * 8 + g), at = line.ct * COLS + col;
-      const __nv_bfloat16 *src = a.q + (int64_t)(line.first + at / a.group) * a.ld_q +
-                                 (int64_t)(line.h * a.group + at % a.group) * HD;
-      uint4 v[HD / 32];
+    for (int i = 0; i < HD / 32; i++) {
+      const int d = BITS == 4 ? (i >> 1) * 64 + cq * 16 + (i & 1) * 8 : i * 32 + cq * 8;
+      v[i] = col < n_cols ? __ldg(reinterpret_cast<const uint4 *>(src + d)) : make_uint4(0, 0, 0, 0);
+    }
 #pragma unroll
-      for (int i = 0; i < HD / 32; i++) {
-        const int d = BITS == 4 ? (i >> 1) * 64 + cq * 16 + (i & 1) * 8 : i * 32 + cq * 8;
-        v[i] = col < n_cols ? __ldg(reinterpret_cast<const uint4 *>(src + d)) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < HD / 32; i++) {
+      if constexpr (BITS == 4) {   // pairs (0, 4), (1, 5), (2, 6), (3, 7), as the codes come
+        qf[4 * i] = __byte_perm(v[i].x, v[i].z, 0x5410);
+        qf[4 * i + 1] = __byte_perm(v[i].x, v[i].z, 0x7632);
+        qf[4 * i + 2] = __byte_perm(v[i].y, v[i].w, 0x5410);
+        qf[4 * i + 3] = __byte_perm(v[i].y, v[i].w, 0x7632);
+      } else {
+        qf[4 * i] = v[i].x, qf[4 * i + 1] = v[i].y, qf[4 * i + 2] = v[i].z, qf[4 * i + 3] = v[i].w;
       }
+    }
+    if constexpr (BITS == 4) {
 #pragma unroll
-      for (int i = 0; i < HD / 32; i++) {
-        if constexpr (BITS == 4) {   // pairs (0, 4), (1, 5), (2, 6), (3, 7), as the codes come
-          qf[nt][4 * i] = __byte_perm(v[i].x, v[i].z, 0x5410);
-          qf[nt][4 * i + 1] = __byte_perm(v[i].x, v[i].z, 0x7632);
-          qf[nt][4 * i + 2] = __byte_perm(v[i].y, v[i].w, 0x5410);
-          qf[nt][4 * i + 3] = __byte_perm(v[i].y, v[i].w, 0x7632);
-        } else {
-          qf[nt][4 * i] = v[i].x, qf[nt][4 * i + 1] = v[i].y, qf[nt][4 * i + 2] = v[i].z, qf[nt][4 * i + 3] = v[i].w;
-        }
-      }
-      if constexpr (BITS == 4) {
+      for (int gr = 0; gr < GR; gr++) {
+        float s = 0.0f;
 #pragma unroll
-        for (int gr = 0; gr < GR; gr++) {
-          float s = 0.0f;
-#pragma unroll
-          for (int i = 8 * gr; i < 8 * gr + 8; i++) s += bf16_lo(qf[nt][i]) + bf16_hi(qf[nt][i]);
-          s += __shfl_xor_sync(0xffffffffu, s, 1);
-          s += __shfl_xor_sync(0xffffffffu, s, 2);
-          qs[gr][nt][0] = __shfl_sync(0xffffffffu, s, 8 * cq);
-          qs[gr][nt][1] = __shfl_sync(0xffffffffu, s, 8 * cq + 4);
-        }
+        for (int i = 8 * gr; i < 8 * gr + 8; i++) s += bf16_lo(qf[i]) + bf16_hi(qf[i]);
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        qs[gr][0] = __shfl_sync(0xffffffffu, s, 8 * cq);
+        qs[gr][1] = __shfl_sync(0xffffffffu, s, 8 * cq + 4);
       }
     }
     // keys that this thread's columns see; the smallest of the unit's columns
-    int lim[NT][2];
+    int lim[2];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const int col = column(nt * 8 + 2 * cq + e), at = line.ct * COLS + col;
-        lim[nt][e] = col < n_cols ? line.len - line.rows + at / a.group + 1 : 0;
-      }
+    for (int e = 0; e < 2; e++) {
+      const int col = column(2 * cq + e), at = line.ct * COLS + col;
+      lim[e] = col < n_cols ? line.len - line.rows + at / a.group + 1 : 0;
+    }
     const int row0 = line.ct * COLS / a.group, row1 = (line.ct * COLS + n_cols - 1) / a.group;
     const int lim_min = line.len - line.rows + row0 + 1;
-    float o[GR * 4][NT][4], l[NT][2], m[NT][2], z[GR][NT][2];
+    float o[GR * 4][4], l[2], m[2], z[GR][2];
 #pragma unroll
     for (int i = 0; i < GR * 4; i++)
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++)
+      for (int e = 0; e < 4; e++) o[i][e] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[i][nt][e] = 0.0f;
+    for (int e = 0; e < 2; e++) {
+      l[e] = 0.0f, m[e] = -INFINITY;
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        l[nt][e] = 0.0f, m[nt][e] = -INFINITY;
-#pragma unroll
-        for (int gr = 0; gr < GR; gr++) z[gr][nt][e] = 0.0f;
-      }
+      for (int gr = 0; gr < GR; gr++) z[gr][e] = 0.0f;
+    }
 
     for (int t = t0; t < t1; t++, it++) {
       const int st = it % STAGES;
@@ -419,13 +412,11 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
         const int in_ring = st * S::TILE;
         const uint8_t *kt = kp + in_ring, *vt = vp + in_ring, *mt = mp + in_ring;
         const int key0 = t * TS + 16 * KS * warp;
-        float sc[KS][NT][4];
+        float sc[KS][4];
 #pragma unroll
         for (int x = 0; x < KS; x++)
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) sc[x][nt][e] = 0.0f;
+          for (int e = 0; e < 4; e++) sc[x][e] = 0.0f;
         if constexpr (BITS == 4) {
 #pragma unroll
           for (int gr = 0; gr < GR; gr++)
@@ -435,28 +426,23 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
               const uint2 u8 = *reinterpret_cast<const uint2 *>(kt + x * 16 * ROW + 8 * ROW + gr * 32);
               const uint32_t m0 = *reinterpret_cast<const uint32_t *>(mt + x * 16 * MARKS + gr * 4);
               const uint32_t m8 = *reinterpret_cast<const uint32_t *>(mt + x * 16 * MARKS + 8 * MARKS + gr * 4);
-              float acc[NT][4];
+              float acc[4];
 #pragma unroll
-              for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[nt][e] = 0.0f;
+              for (int e = 0; e < 4; e++) acc[e] = 0.0f;
 #pragma unroll
               for (int i = 0; i < 4; i++) {
                 const uint32_t x0 = i < 2 ? u0.x : u0.y, x8 = i < 2 ? u8.x : u8.y;
                 const int j = 2 * (i & 1);
                 const uint32_t af[4] = {codes128(x0, j), codes128(x8, j), codes128(x0, j + 1), codes128(x8, j + 1)};
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) mma_bf16(acc[nt], af, qf[nt][8 * gr + 2 * i], qf[nt][8 * gr + 2 * i + 1]);
+                mma_bf16(acc, af, qf[8 * gr + 2 * i], qf[8 * gr + 2 * i + 1]);
               }
               const float s0 = bf16_lo(m0), s8 = bf16_lo(m8);
               const float b0 = fmaf(-128.0f, s0, bf16_hi(m0)), b8 = fmaf(-128.0f, s8, bf16_hi(m8));
 #pragma unroll
-              for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                  sc[x][nt][e] = fmaf(s0, acc[nt][e], fmaf(b0, qs[gr][nt][e], sc[x][nt][e]));
-                  sc[x][nt][2 + e] = fmaf(s8, acc[nt][2 + e], fmaf(b8, qs[gr][nt][e], sc[x][nt][2 + e]));
-                }
+              for (int e = 0; e < 2; e++) {
+                sc[x][e] = fmaf(s0, acc[e], fmaf(b0, qs[gr][e], sc[x][e]));
+                sc[x][2 + e] = fmaf(s8, acc[2 + e], fmaf(b8, qs[gr][e], sc[x][2 + e]));
+              }
             }
         } else {
 #pragma unroll
@@ -466,11 +452,8 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
               const uint4 x0 = *reinterpret_cast<const uint4 *>(kt + x * 16 * ROW + i * 64);
               const uint4 x8 = *reinterpret_cast<const uint4 *>(kt + x * 16 * ROW + 8 * ROW + i * 64);
               const uint32_t a0[4] = {x0.x, x8.x, x0.y, x8.y}, a1[4] = {x0.z, x8.z, x0.w, x8.w};
-#pragma unroll
-              for (int nt = 0; nt < NT; nt++) {
-                mma_bf16(sc[x][nt], a0, qf[nt][4 * i], qf[nt][4 * i + 1]);
-                mma_bf16(sc[x][nt], a1, qf[nt][4 * i + 2], qf[nt][4 * i + 3]);
-              }
+              mma_bf16(sc[x], a0, qf[4 * i], qf[4 * i + 1]);
+              mma_bf16(sc[x], a1, qf[4 * i + 2], qf[4 * i + 3]);
             }
         }
         // tokens that a column does not see, or that are not there
@@ -481,55 +464,47 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
 #pragma unroll
           for (int x = 0; x < KS; x++)
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-              for (int e = 0; e < 4; e++) {
-                const int r = e < 2 ? g : g + 8;
-                if (!(bits[x] >> r & 1) || key0 + 16 * x + r >= lim[nt][e & 1]) sc[x][nt][e] = -INFINITY;
-              }
+            for (int e = 0; e < 4; e++) {
+              const int r = e < 2 ? g : g + 8;
+              if (!(bits[x] >> r & 1) || key0 + 16 * x + r >= lim[e & 1]) sc[x][e] = -INFINITY;
+            }
         }
         // the running maximum moves only where a column grows past it by 2^8 (a weight of up to 2^8 costs an f32 sum
         // nothing): most tiles then skip the reduction and the rescaling
-        float top[NT][2];
+        float top[2];
         bool grows = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int e = 0; e < 2; e++) {
+          top[e] = fmaxf(sc[0][e], sc[0][2 + e]);
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            top[nt][e] = fmaxf(sc[0][nt][e], sc[0][nt][2 + e]);
-#pragma unroll
-            for (int x = 1; x < KS; x++) top[nt][e] = fmaxf(top[nt][e], fmaxf(sc[x][nt][e], sc[x][nt][2 + e]));
-            grows |= top[nt][e] * a.scale_log2 > m[nt][e] + 8.0f;
-          }
+          for (int x = 1; x < KS; x++) top[e] = fmaxf(top[e], fmaxf(sc[x][e], sc[x][2 + e]));
+          grows |= top[e] * a.scale_log2 > m[e] + 8.0f;
+        }
         if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++)
+          for (int e = 0; e < 2; e++) {
+            float v = fmaxf(top[e] * a.scale_log2, m[e]);
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-              float v = fmaxf(top[nt][e] * a.scale_log2, m[nt][e]);
+            for (int y = 4; y < 32; y <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, y));
+            const float f = v == -INFINITY ? 1.0f : ex2(m[e] - v);
+            m[e] = v;
+            l[e] *= f;
 #pragma unroll
-              for (int y = 4; y < 32; y <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, y));
-              const float f = v == -INFINITY ? 1.0f : ex2(m[nt][e] - v);
-              m[nt][e] = v;
-              l[nt][e] *= f;
+            for (int gr = 0; gr < GR; gr++) z[gr][e] *= f;
 #pragma unroll
-              for (int gr = 0; gr < GR; gr++) z[gr][nt][e] *= f;
-#pragma unroll
-              for (int i = 0; i < GR * 4; i++) o[i][nt][e] *= f, o[i][nt][2 + e] *= f;
-            }
+            for (int i = 0; i < GR * 4; i++) o[i][e] *= f, o[i][2 + e] *= f;
+          }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int e = 0; e < 2; e++) {
+          const float mm = m[e] == -INFINITY ? 0.0f : m[e];
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const float mm = m[nt][e] == -INFINITY ? 0.0f : m[nt][e];
-#pragma unroll
-            for (int x = 0; x < KS; x++) {
-              sc[x][nt][e] = ex2(fmaf(sc[x][nt][e], a.scale_log2, -mm));
-              sc[x][nt][2 + e] = ex2(fmaf(sc[x][nt][2 + e], a.scale_log2, -mm));
-              l[nt][e] += sc[x][nt][e] + sc[x][nt][2 + e];
-            }
+          for (int x = 0; x < KS; x++) {
+            sc[x][e] = ex2(fmaf(sc[x][e], a.scale_log2, -mm));
+            sc[x][2 + e] = ex2(fmaf(sc[x][2 + e], a.scale_log2, -mm));
+            l[e] += sc[x][e] + sc[x][2 + e];
           }
+        }
         if constexpr (BITS == 4) {
 #pragma unroll
           for (int gr = 0; gr < GR; gr++)
@@ -544,32 +519,29 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
               const uint32_t wd = *reinterpret_cast<const uint32_t *>(vc + 9 * ROW);
               const float s0 = bf16_lo(m0), s8 = bf16_lo(m8);
               const float b0 = fmaf(-16.0f, s0, bf16_hi(m0)), b8 = fmaf(-16.0f, s8, bf16_hi(m8));
-              uint32_t p0[NT], p8[NT], r0[NT], r8[NT];
+              uint32_t p0, p8, r0, r8;
+              float w[4];
+              if (!edge) {
 #pragma unroll
-              for (int nt = 0; nt < NT; nt++) {
-                float w[4];
-                if (!edge) {
-#pragma unroll
-                  for (int e = 0; e < 2; e++) {
-                    w[e] = sc[x][nt][e] * s0, w[2 + e] = sc[x][nt][2 + e] * s8;
-                    z[gr][nt][e] = fmaf(sc[x][nt][e], b0, fmaf(sc[x][nt][2 + e], b8, z[gr][nt][e]));
-                  }
-                } else {   // a weight of zero leaves out whatever the token holds
-#pragma unroll
-                  for (int e = 0; e < 2; e++) {
-                    const bool k0 = sc[x][nt][e] != 0.0f, k8 = sc[x][nt][2 + e] != 0.0f;
-                    w[e] = k0 ? sc[x][nt][e] * s0 : 0.0f, w[2 + e] = k8 ? sc[x][nt][2 + e] * s8 : 0.0f;
-                    if (k0) z[gr][nt][e] += sc[x][nt][e] * b0;
-                    if (k8) z[gr][nt][e] += sc[x][nt][2 + e] * b8;
-                  }
+                for (int e = 0; e < 2; e++) {
+                  w[e] = sc[x][e] * s0, w[2 + e] = sc[x][2 + e] * s8;
+                  z[gr][e] = fmaf(sc[x][e], b0, fmaf(sc[x][2 + e], b8, z[gr][e]));
                 }
-                if constexpr (DUAL) {
-                  p0[nt] = split_columns(w[0], w[1], cq >= 2);
-                  p8[nt] = split_columns(w[2], w[3], cq >= 2);
-                } else {
-                  split_weights(w[0], w[1], p0[nt], r0[nt]);
-                  split_weights(w[2], w[3], p8[nt], r8[nt]);
+              } else {   // a weight of zero leaves out whatever the token holds
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                  const bool k0 = sc[x][e] != 0.0f, k8 = sc[x][2 + e] != 0.0f;
+                  w[e] = k0 ? sc[x][e] * s0 : 0.0f, w[2 + e] = k8 ? sc[x][2 + e] * s8 : 0.0f;
+                  if (k0) z[gr][e] += sc[x][e] * b0;
+                  if (k8) z[gr][e] += sc[x][2 + e] * b8;
                 }
+              }
+              if constexpr (DUAL) {
+                p0 = split_columns(w[0], w[1], cq >= 2);
+                p8 = split_columns(w[2], w[3], cq >= 2);
+              } else {
+                split_weights(w[0], w[1], p0, r0);
+                split_weights(w[2], w[3], p8, r8);
               }
               const uint32_t lo[2] = {__byte_perm(wa, wb, 0x5410), __byte_perm(wa, wb, 0x7632)};
               const uint32_t hi[2] = {__byte_perm(wc, wd, 0x5410), __byte_perm(wc, wd, 0x7632)};
@@ -578,11 +550,8 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
                 const int i = 2 * (j & 1);
                 const uint32_t af[4] = {codes16(lo[j >> 1], i), codes16(lo[j >> 1], i + 1), codes16(hi[j >> 1], i),
                                         codes16(hi[j >> 1], i + 1)};
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                  mma_bf16(o[4 * gr + j][nt], af, p0[nt], p8[nt]);
-                  if constexpr (!DUAL) mma_bf16(o[4 * gr + j][nt], af, r0[nt], r8[nt]);
-                }
+                mma_bf16(o[4 * gr + j], af, p0, p8);
+                if constexpr (!DUAL) mma_bf16(o[4 * gr + j], af, r0, r8);
               }
             }
         } else {
@@ -590,12 +559,9 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
 #pragma unroll
           for (int x = 0; x < KS; x++) {
             const uint8_t *vc = vt + x * 16 * ROW;
-            uint32_t p0[NT], p8[NT], r0[NT], r8[NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-              split_weights(sc[x][nt][0], sc[x][nt][1], p0[nt], r0[nt]);
-              split_weights(sc[x][nt][2], sc[x][nt][3], p8[nt], r8[nt]);
-            }
+            uint32_t p0, p8, r0, r8;
+            split_weights(sc[x][0], sc[x][1], p0, r0);
+            split_weights(sc[x][2], sc[x][3], p8, r8);
 #pragma unroll
             for (int gr = 0; gr < GR; gr++) {
               uint4 v[4];
@@ -607,11 +573,8 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
                   const uint32_t wa = (&v[0].x)[j], wb = (&v[1].x)[j], wc = (&v[2].x)[j], wd = (&v[3].x)[j];
                   const uint32_t af[4] = {__byte_perm(wa, wb, 0x5410), __byte_perm(wa, wb, 0x7632),
                                           __byte_perm(wc, wd, 0x5410), __byte_perm(wc, wd, 0x7632)};
-#pragma unroll
-                  for (int nt = 0; nt < NT; nt++) {
-                    mma_bf16(o[4 * gr + j][nt], af, p0[nt], p8[nt]);
-                    mma_bf16(o[4 * gr + j][nt], af, r0[nt], r8[nt]);
-                  }
+                  mma_bf16(o[4 * gr + j], af, p0, p8);
+                  mma_bf16(o[4 * gr + j], af, r0, r8);
                 }
               } else {
                 // row by row: a token that a row does not see is zeros to it, and another row's product, where that
@@ -628,15 +591,12 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
                     const uint32_t wc = (&v[2].x)[j] & keep[2], wd = (&v[3].x)[j] & keep[3];
                     const uint32_t af[4] = {__byte_perm(wa, wb, 0x5410), __byte_perm(wa, wb, 0x7632),
                                             __byte_perm(wc, wd, 0x5410), __byte_perm(wc, wd, 0x7632)};
+                    float tmp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    mma_bf16(tmp, af, p0, p8);
+                    mma_bf16(tmp, af, r0, r8);
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                      float tmp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                      mma_bf16(tmp, af, p0[nt], p8[nt]);
-                      mma_bf16(tmp, af, r0[nt], r8[nt]);
-#pragma unroll
-                      for (int e = 0; e < 4; e++)
-                        if (lim[nt][e & 1] == seen) o[4 * gr + j][nt][e] += tmp[e];
-                    }
+                    for (int e = 0; e < 4; e++)
+                      if (lim[e & 1] == seen) o[4 * gr + j][e] += tmp[e];
                   }
                 }
               }
@@ -651,44 +611,40 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
     // ---- the warps' parts of the unit joined
     const bool mine = !DUAL || cq < 2;   // this thread's columns are query columns
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
+    for (int e = 0; e < 2; e++) {
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
+      for (int x = 4; x < 32; x <<= 1) {
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
+        if constexpr (BITS == 4) {
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) {
-          l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
-          if constexpr (BITS == 4) {
-#pragma unroll
-            for (int gr = 0; gr < GR; gr++) z[gr][nt][e] += __shfl_xor_sync(0xffffffffu, z[gr][nt][e], x);
-          }
+          for (int gr = 0; gr < GR; gr++) z[gr][e] += __shfl_xor_sync(0xffffffffu, z[gr][e], x);
         }
-        if (g == 0 && mine) wm[warp][nt * 8 + 2 * cq + e] = m[nt][e], wl[warp][nt * 8 + 2 * cq + e] = l[nt][e];
       }
+      if (g == 0 && mine) wm[warp][2 * cq + e] = m[e], wl[warp][2 * cq + e] = l[e];
+    }
     const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory"); };
     sync();
-    float f[NT][2];
+    float f[2];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
+    for (int e = 0; e < 2; e++) {
+      const int col = column(2 * cq + e);
+      float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const int col = column(nt * 8 + 2 * cq + e);
-        float top = -INFINITY, sum = 0.0f;
+      for (int i = 0; i < NW; i++) top = fmaxf(top, wm[i][col]);
 #pragma unroll
-        for (int i = 0; i < NW; i++) top = fmaxf(top, wm[i][col]);
-#pragma unroll
-        for (int i = 0; i < NW; i++) sum += wm[i][col] == -INFINITY ? 0.0f : wl[i][col] * ex2(wm[i][col] - top);
-        f[nt][e] = m[nt][e] == -INFINITY ? 0.0f : ex2(m[nt][e] - top);
-        if (warp == 0 && g == 0 && mine) um[col] = top, ul[col] = sum;
-      }
+      for (int i = 0; i < NW; i++) sum += wm[i][col] == -INFINITY ? 0.0f : wl[i][col] * ex2(wm[i][col] - top);
+      f[e] = m[e] == -INFINITY ? 0.0f : ex2(m[e] - top);
+      if (warp == 0 && g == 0 && mine) um[col] = top, ul[col] = sum;
+    }
     // where the piece ends inside the unit, or began inside it: a part
     const bool whole = t0 == 0 && t1 == line.tiles;
     float *part = a.parts + ((int64_t)me * 2 + (t0 == 0)) * S::PART;
     // an accumulator tile's values: dimensions d, d + 1 of columns 2 cq, 2 cq + 1
-    const auto put = [&](int i, int nt, float4 v) {
+    const auto put = [&](int i, float4 v) {
       const int d = (i >> 2) * 64 + 8 * g + 2 * (i & 3);
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        const int col = nt * 8 + 2 * cq + e, at = line.ct * COLS + col;
+        const int col = 2 * cq + e, at = line.ct * COLS + col;
         if (!mine || col >= n_cols) continue;
         const float inv = ul[col] > 0.0f ? 1.0f / ul[col] : ul[col] == 0.0f ? 0.0f : ul[col];
         *reinterpret_cast<uint32_t *>(a.out + ((int64_t)(line.first + at / a.group) * a.heads + line.h * a.group + at % a.group) * HD + d) =
@@ -701,14 +657,14 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
       for (int ch = 0; ch < S::ACC / S::CHUNK; ch++) {
 #pragma unroll
         for (int k = 0; k < S::CHUNK; k++) {
-          const int i = (ch * S::CHUNK + k) / NT, nt = (ch * S::CHUNK + k) % NT;
+          const int i = ch * S::CHUNK + k;
           float v[4];
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            v[e] = o[i][nt][e];
+            v[e] = o[i][e];
             if constexpr (DUAL) v[e] += __shfl_xor_sync(0xffffffffu, v[e], 2);
-            if constexpr (BITS == 4) v[e] += z[i >> 2][nt][e & 1];
-            v[e] = f[nt][e & 1] == 0.0f ? 0.0f : v[e] * f[nt][e & 1];
+            if constexpr (BITS == 4) v[e] += z[i >> 2][e & 1];
+            v[e] = f[e & 1] == 0.0f ? 0.0f : v[e] * f[e & 1];
           }
           if (used) red[(warp * S::CHUNK + k) * 32 + lane] = make_float4(v[0], v[1], v[2], v[3]);
         }
@@ -721,7 +677,7 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
             const float4 u = red[(x * S::CHUNK + warp) * 32 + lane];
             v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
           }
-          if (last) put(at / NT, at % NT, v);
+          if (last) put(at, v);
           else __stcg(reinterpret_cast<float4 *>(part) + at * 32 + lane, v);
         }
         sync();
@@ -761,15 +717,13 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
         if (lane == 0) um[col] = all, ul[col] = sum;
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++)
+      for (int e = 0; e < 2; e++) {
+        f[e] = 1.0f;
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          f[nt][e] = 1.0f;
+        for (int gr = 0; gr < GR; gr++) z[gr][e] = 0.0f;
 #pragma unroll
-          for (int gr = 0; gr < GR; gr++) z[gr][nt][e] = 0.0f;
-#pragma unroll
-          for (int i = 0; i < GR * 4; i++) o[i][nt][e] = o[i][nt][2 + e] = 0.0f;
-        }
+        for (int i = 0; i < GR * 4; i++) o[i][e] = o[i][2 + e] = 0.0f;
+      }
       for (int x0 = c0; x0 <= c1; x0 += kBatch) {
         const int n = min(kBatch, c1 - x0 + 1);
         sync();
@@ -797,10 +751,10 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
               const int y = min(x + k * NW * SIDES, n - 1);
 #pragma unroll
               for (int j = 0; j < S::ACC; j++) {
-                const int i = j / NT, nt = j % NT, col = column(nt * 8 + 2 * cq);
+                const int col = column(2 * cq);
                 const float f0 = weights[y * COLS + col], f1 = weights[y * COLS + col + 1];
-                if (f0 != 0.0f) o[i][nt][0] += u[k][j].x * f0, o[i][nt][2] += u[k][j].z * f0;
-                if (f1 != 0.0f) o[i][nt][1] += u[k][j].y * f1, o[i][nt][3] += u[k][j].w * f1;
+                if (f0 != 0.0f) o[j][0] += u[k][j].x * f0, o[j][2] += u[k][j].z * f0;
+                if (f1 != 0.0f) o[j][1] += u[k][j].y * f1, o[j][3] += u[k][j].w * f1;
               }
             }
           }
@@ -838,20 +792,13 @@ int launch(const PagedView &v, AttnParams &p, const Sm100PagedAttnArgs *a, cudaS
   return launch_status("paged_attention");
 }
 
-// Query columns of a unit: the fewest that hold a sequence's rows and heads of a group, at most 16 (8 at 256 dimensions, where
-// the accumulators of 16 would not fit the registers).
-int columns_of(int head_dim, int bits, int64_t cols) {
-  return cols > 8 && head_dim <= 128 ? 16 : cols > 4 || bits == 16 ? 8 : 4;
-}
+// Query columns of a unit
+int columns_of(int bits, int64_t cols) { return cols > 4 || bits == 16 ? 8 : 4; }
 
 template <int HD, int BITS>
 int launch_columns(const PagedView &v, AttnParams &p, const Sm100PagedAttnArgs *a, cudaStream_t st) {
-  const int cols = columns_of(HD, BITS, (int64_t)a->max_rows * p.group);
-  if constexpr (HD <= 128) {
-    if (cols == 16) return launch<HD, BITS, 16>(v, p, a, st);
-  }
   if constexpr (BITS == 4) {
-    if (cols == 4) return launch<HD, BITS, 4>(v, p, a, st);
+    if (columns_of(BITS, (int64_t)a->max_rows * p.group) == 4) return launch<HD, BITS, 4>(v, p, a, st);
   }
   return launch<HD, BITS, 8>(v, p, a, st);
 }
@@ -861,8 +808,8 @@ int launch_columns(const PagedView &v, AttnParams &p, const Sm100PagedAttnArgs *
 extern "C" uint64_t sm100_paged_attention_ws_bytes(const Sm100PagedCache *c, int32_t heads, int32_t max_rows) {
   PagedView v;
   if (sm100_paged_view(c, "paged_attention_ws_bytes", &v) || heads < 1 || heads % c->kv_heads || max_rows < 1) return 0;
-  const uint64_t cols = columns_of(c->head_dim, c->bits, (int64_t)max_rows * (heads / c->kv_heads));
-  return kMaxPieces * 4 + (uint64_t)kMaxPieces * 2 * ((cols < 8 ? 8 : cols) * c->head_dim + 2 * cols) * 4;
+  const uint64_t cols = columns_of(c->bits, (int64_t)max_rows * (heads / c->kv_heads));
+  return kMaxPieces * 4 + (uint64_t)kMaxPieces * 2 * (8 * c->head_dim + 2 * cols) * 4;
 }
 
 extern "C" int sm100_paged_attention(const Sm100PagedCache *c, const Sm100PagedAttnArgs *a, void *stream) {
