@@ -4,8 +4,13 @@
 //
 // What bounds it: every key and value is read once for up to 8 query columns
 // (the heads of a group times the new rows), so a decode step is bound by
-// memory, and in 4 bits, where a token of 128 + 128 dimensions is 144 bytes, by
-// issue slots next to it (unpacking, about one instruction a value).
+// memory: bf16 pages stream at 5.5 TB/s (16 sequences of 4096, 8 key heads of
+// 128: 49 us).  In 4 bits, where a token of 128 + 128 dimensions is 144 bytes,
+// issue and the half-rate integer pipe bind first: unpacking takes some 150 of
+// the 365 instructions that a warp spends on 16 tokens (64 sequences of up to
+// 16384: 138 us, 3.8 TB/s, 57 % of the issue slots, 58 % of the integer pipe).
+// Short calls are bound by the chain lengths -> cut -> table -> first tile ->
+// joining (one sequence of 32768 in 4 bits: 24 us, 12 of them streaming).
 //
 // Split.  The tiles (TS tokens) of all units (sequence, key head, 8 query
 // columns) form one line that is cut into gridDim equal pieces, one per CTA, so
@@ -138,7 +143,9 @@ __device__ __forceinline__ uint32_t codes16(uint32_t w, int i) {
 
 // The line: units in the order (sequence, key head, column tile), each kPad
 // places for what a unit costs beside its tiles (queries, joining, output:
-// about that many tiles' time), then its token tiles.
+// about that many tiles' time), then its token tiles.  1, 2, 3, 4 places: 64
+// sequences of up to 16384 take 145, 138, 139, 140 us, 8 of up to 4096 with 4 new
+// rows 34.8, 34.1, 35.5, 36.4.
 constexpr int kPad = 2;
 
 template <int TS, int NC>

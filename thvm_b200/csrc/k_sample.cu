@@ -12,9 +12,11 @@
 // The kept id with the largest d - ln(noise) wins: -ln of an exponential number
 // is a Gumbel number, so id i wins with probability w_i / sum w.
 //
-// What bounds it: the logits once (and the random numbers of the kept ids);
-// then some ten instructions an id and pass and, with few rows, the latency of
-// the steps one after the other.  A row belongs to one CTA, or with few rows to
+// What bounds it: the logits once (and the random numbers of the kept ids) is the
+// floor; above it, with many rows some ten to twenty instructions an id and pass
+// (256 x 102400 bf16: 79 us, 8 for the bytes; rows that keep tens of thousands of
+// ids take longest), with few rows the latency of the steps one after the other
+// (one row of 50257: 16 us, 32 of 102400: 29.5).  A row belongs to one CTA, or with few rows to
 // a cluster of 4 or 8 that holds it in shared memory where it fits (later passes
 // come from L2 otherwise).  A cut is found without sorting the row:
 //   1. a histogram of (l_max - l) / T in 4096 bins of 1/128 of the ids that can
@@ -23,9 +25,9 @@
 //      ids weigh count * e^-bin within e^(+-1/256), which bounds the cut to some
 //      bins, and where those hold too many ids, narrower bounds about a guess
 //      that knows the row's whole weight;
-//   3. one pass sums what lies above those bins and gathers their ids (a few
-//      hundred), which CTA 0 sorts and scans; a guess that missed is put right
-//      by what the pass summed.
+//   3. one pass gathers the ids of those bins (a few hundred), among which CTA 0
+//      selects, sums what lies above them, which is kept, and runs its race; a
+//      guess that missed is put right by what the pass summed.
 // Where everything above the cut fits in the list too (top-k of up to some
 // hundreds, a peaked top-p) the list is all that is kept, and CTA 0 runs the
 // race on it alone.  A bin that overflows the list (thousands of equal logits at
@@ -789,8 +791,8 @@ cudaError_t launch(const SampleParams &p, int B, cudaStream_t st) {
 }
 
 // CTAs of a row.  A row's passes are bound by its SM where there are many rows (one CTA each, two an SM), by the cluster's
-// exchanges where there are few: 256 x 102400 bf16 takes 87, 98, 189 us with 1, 4, 8 CTAs a row, 32 x 102400 f32 71, 38,
-// 34 us, one row of 50257 28, 18, 18 us.
+// exchanges where there are few: 256 x 102400 bf16 took 87, 98, 189 us with 1, 4, 8 CTAs a row, 32 x 102400 f32 71, 38,
+// 34 us, one row of 50257 28, 18, 18 us (when the rule was set; each has become faster since).
 template <typename In>
 cudaError_t launch_row(SampleParams p, int B, cudaStream_t st) {
   const int C = 8 * B <= 2 * 148 && p.V > 8 * 1024 ? 8 : B <= 148 && p.V > 4 * 1024 ? 4 : 1;
