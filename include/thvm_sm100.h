@@ -723,8 +723,8 @@ uint32_t sm100_attn_prefill_status(void);
  *                  byte i, 2 i + 1 in the high half), then bf16 (scale,
  *                  minimum) pairs [page][head_dim / 64][2]: a code c of a group
  *                  of 64 dimensions stands for minimum + c * scale
- * (a page and head is one contiguous block, so attention brings it in by one
- * bulk copy).  table [n_seq][max_pages] (device) is the page of each page slot
+ * (a page and head is one contiguous block, so attention brings each of its
+ * areas in by one bulk copy).  table [n_seq][max_pages] (device) is the page of each page slot
  * of a sequence: token p of sequence s is row p % page of page
  * table[s][p / page].  page 16, 32 or 64; head_dim 64, 128 or 256; pool
  * 16-byte aligned. */

@@ -17,9 +17,10 @@
 // heads, the next head's load under way.
 //
 // What bounds it: for many rows memory and issue about alike (16384 rows of 16 +
-// 2 x 16 heads of 128, bf16: 91 us, 4.5 TB/s read and written, 150 instructions a
-// warp and step at 68 % of the issue slots; a second step's load under way
-// changes nothing), for few the latency of seq -> page -> store.
+// 2 x 16 heads of 128, bf16: 91 us, 4.5 TB/s read and written, 151 instructions a
+// warp and step at 64 % of the issue slots; a second step's load under way
+// changes nothing), in 4 bits issue (4093 rows of 28 + 2 x 4 heads: 27 us under
+// the profiler, 70 % of the slots), for few the latency of seq -> page -> store.
 #include "paged.cuh"
 
 using namespace sm100;

@@ -6,11 +6,12 @@
 // (the heads of a group times the new rows), so a decode step is bound by
 // memory: bf16 pages stream at 5.5 TB/s (16 sequences of 4096, 8 key heads of
 // 128: 49 us).  In 4 bits, where a token of 128 + 128 dimensions is 144 bytes,
-// issue and the half-rate integer pipe bind first: unpacking takes some 150 of
-// the 365 instructions that a warp spends on 16 tokens (64 sequences of up to
-// 16384: 138 us, 3.8 TB/s, 57 % of the issue slots, 58 % of the integer pipe).
-// Short calls are bound by the chain lengths -> cut -> table -> first tile ->
-// joining (one sequence of 32768 in 4 bits: 24 us, 12 of them streaming).
+// issue and the integer pipe bind first: of the 365 instructions for 16 tokens
+// 137 are the shifts and ANDs that unpack (16 sequences of 16384: 57 % of the
+// issue slots and 58 % of the integer pipe, memory at 42 %; 64 of up to 16384:
+// 139 us, 3.8 TB/s).  Short calls are bound by the chain lengths -> cut -> table
+// -> first tile and by the joining (one sequence of 32768 in 4 bits, 24 us: tiles
+// done after 7 to 15, the last unit joined 10 later).
 //
 // Split.  The tiles (TS tokens) of all units (sequence, key head, 8 query
 // columns) form one line that is cut into gridDim equal pieces, one per CTA, so

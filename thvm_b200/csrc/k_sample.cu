@@ -13,12 +13,13 @@
 // is a Gumbel number, so id i wins with probability w_i / sum w.
 //
 // What bounds it: the logits once (and the random numbers of the kept ids) is the
-// floor; above it, with many rows some ten to twenty instructions an id and pass
-// (256 x 102400 bf16: 79 us, 8 for the bytes; rows that keep tens of thousands of
-// ids take longest), with few rows the latency of the steps one after the other
-// (one row of 50257: 16 us, 32 of 102400: 29.5).  A row belongs to one CTA, or with few rows to
-// a cluster of 4 or 8 that holds it in shared memory where it fits (later passes
-// come from L2 otherwise).  A cut is found without sorting the row:
+// floor; above it, with many rows the slowest row (256 x 102400 bf16: 79 to 88 us
+// with the draw of the settings, 8 for the bytes, 32 instructions an id over all
+// passes; a traced row takes 35 us on average, the longest 66), with few rows the
+// latency of the steps one after the other (one row of 50257: 16 us, 32 of 102400:
+// 30 to 32).  A row belongs to one CTA, or with few rows to a cluster of 4 or 8
+// that holds it in shared memory where it fits (later passes come from L2
+// otherwise).  A cut is found without sorting the row:
 //   1. a histogram of (l_max - l) / T in 4096 bins of 1/128 of the ids that can
 //      be chosen at all, summed over the cluster slice by slice;
 //   2. the bins that can hold the cut: by count it is one; by weight a bin's
@@ -791,8 +792,8 @@ cudaError_t launch(const SampleParams &p, int B, cudaStream_t st) {
 }
 
 // CTAs of a row.  A row's passes are bound by its SM where there are many rows (one CTA each, two an SM), by the cluster's
-// exchanges where there are few: 256 x 102400 bf16 took 87, 98, 189 us with 1, 4, 8 CTAs a row, 32 x 102400 f32 71, 38,
-// 34 us, one row of 50257 28, 18, 18 us (when the rule was set; each has become faster since).
+// exchanges where there are few: with 1, 4, 8 CTAs a row 256 x 102400 bf16 takes 79 to 88, 93, 164 us, 32 x 102400 f32
+// 62 to 76, 35 to 38, 30 to 32, one row of 50257 24.8, 16.8, 16.4 (two draws of the settings).
 template <typename In>
 cudaError_t launch_row(SampleParams p, int B, cudaStream_t st) {
   const int C = 8 * B <= 2 * 148 && p.V > 8 * 1024 ? 8 : B <= 148 && p.V > 4 * 1024 ? 4 : 1;
