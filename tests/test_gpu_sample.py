@@ -184,6 +184,58 @@ def test_many_rows_on_every_cluster_size_repeat_to_the_bit():
         assert torch.equal(t, tok[:n]) and float((lp - logp[:n]).abs().max()) <= 1e-5
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("B,V", [(34, 33333), (35, 33333), (70, 8200), (72, 33333), (100, 2049), (101, 50257), (148, 9001),
+                                 (149, 33333)])
+def test_draws_around_the_changes_of_launch_shape(B, V, bf16):
+    """Ids and log-probabilities where another number of CTAs takes a row, and where a part is hardly worth one.
+
+    The tolerances are those of whole batches above: the sums are over as many weights or fewer."""
+    import torch
+    rng = np.random.default_rng(B + V + bf16)
+    x = (2.5 * rng.standard_normal((B, V))).astype(np.float32)
+    x[rng.random(x.shape) < 0.2] = -np.inf
+    x[:, V - 1] = 1.0
+    noise = rng.exponential(size=(B, V)).astype(np.float32)
+    T = rng.uniform(0.4, 1.5, B).astype(np.float32)
+    k = rng.choice([0, 1, 20, 64, 500, 2000, V], B).astype(np.int32)
+    p = rng.choice([1.0, 0.95, 0.9, 0.5], B).astype(np.float32)
+    m = rng.choice([0.0, 0.0, 0.02], B).astype(np.float32)
+    xt = torch.from_numpy(x).cuda()
+    xt = xt.bfloat16() if bf16 else xt
+    d = lambda a: torch.from_numpy(a).cuda()
+    tok, logp = _sampler()(xt, d(noise), temperature=d(T), top_k=d(k), top_p=d(p), min_p=d(m))
+    tok, logp, x = tok.cpu().numpy(), logp.cpu().numpy(), xt.double().cpu().numpy()
+    for b in range(B):
+        ids, dd = _kept(x[b], np.float64(T[b]), int(k[b]), np.float64(p[b]), np.float64(m[b]))
+        score = dd - np.log(noise[b, ids].astype(np.float64))
+        at = np.nonzero(ids == tok[b])[0]
+        assert len(at) == 1, (b, tok[b])
+        assert score[at[0]] >= score.max() - 1e-5
+        assert abs(logp[b] - (dd[at[0]] - np.log(np.exp(dd).sum()))) <= 1e-5 * (1 + abs(dd[at[0]]))
+
+
+@pytest.mark.parametrize("kind", list(ROWS))
+def test_kept_set_in_pairs_of_ctas(kind):
+    """A hundred copies of a row, one id's random number nearly zero in each: that id is chosen exactly where top-k keeps it."""
+    import torch
+    V, B = 30011, 100
+    rng = np.random.default_rng(5)
+    row = ROWS[kind](V, rng)
+    if not (row > -np.inf).any():
+        row[V // 2] = 0.5
+    order, d = _kept(row.astype(np.float64), 1.0, None, None, None)
+    # an id far below the largest needs a random number whose logarithm reaches that far: only those are asked
+    order = order[d > -85]
+    x = torch.from_numpy(row).cuda().expand(B, V).contiguous()
+    for k in (1, 20, 700, 4000):
+        asked = [min(max(0, min(k, len(order)) - B // 2 + i), len(order) - 1) for i in range(B)]
+        noise = torch.ones(B, V, device="cuda")
+        noise[torch.arange(B), torch.from_numpy(order[asked].copy()).cuda()] = 1e-38
+        got = _run(x, noise, k=k)[0].cpu().numpy()
+        assert (got == np.where(np.array(asked) < k, order[asked], order[0])).all(), (kind, k)
+
+
 def test_probabilities_of_the_draw():
     """20000 draws over 12 ids with top-p: frequencies within 5 standard deviations of the kept ids' probabilities,
     none of the others."""

@@ -17,7 +17,7 @@
 // with the draw of the settings, 8 for the bytes, 32 instructions an id over all
 // passes; a traced row takes 35 us on average, the longest 66), with few rows the
 // latency of the steps one after the other (one row of 50257: 16 us, 32 of 102400:
-// 30 to 32).  A row belongs to one CTA, or with few rows to a cluster of 4 or 8
+// 30 to 32).  A row belongs to one CTA, or with few rows to a cluster of 2 to 8
 // that holds it in shared memory where it fits (later passes come from L2
 // otherwise).  A cut is found without sorting the row:
 //   1. a histogram of (l_max - l) / T in 4096 bins of 1/128 of the ids that can
@@ -764,44 +764,77 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
 
 constexpr int kHeld = 64 * 1024;   // bytes of a row that a CTA holds: two CTAs an SM
 
+// A launch of B clusters of C CTAs
 template <typename In, bool RESIDENT, int C>
-cudaError_t launch(const SampleParams &p, int B, cudaStream_t st) {
-  static bool ready[64];
-  const auto kernel = sample_kernel<In, RESIDENT, C>;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (RESIDENT && (dev >= 64 || !ready[dev])) {
-    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeld)) != cudaSuccess) return e;
-    if (dev < 64) ready[dev] = true;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(B * C));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = RESIDENT ? (p.chunk * sizeof(In) + 15) / 16 * 16 : 0;
-  cfg.stream = st;
+struct Launch {
   cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = C;
-  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = C > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  cudaLaunchConfig_t cfg = {};
+  Launch(int B, size_t dynamic, cudaStream_t st) {
+    cfg.gridDim = dim3((unsigned)(B * C));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = dynamic;
+    cfg.stream = st;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = C;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = C > 1 ? 2 : 1;
+  }
+};
+
+// Clusters of C CTAs that the device holds at once, asked for once a device (the largest shared memory that a launch takes);
+// *e tells of a call that failed
+template <typename In, bool RESIDENT, int C>
+int clusters_at_once(cudaError_t *e) {
+  static int known[64];   // clusters + 1
+  const auto kernel = sample_kernel<In, RESIDENT, C>;
+  int dev = 0, n = 0;
+  if ((*e = cudaGetDevice(&dev)) != cudaSuccess) return 0;
+  if (dev < 64 && known[dev]) return known[dev] - 1;
+  if (RESIDENT && (*e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeld)) != cudaSuccess) return 0;
+  Launch<In, RESIDENT, C> one(1, RESIDENT ? kHeld : 0, nullptr);
+  one.at[0] = one.at[1];
+  one.cfg.numAttrs = 1;
+  if ((*e = cudaOccupancyMaxActiveClusters(&n, kernel, &one.cfg)) != cudaSuccess) return 0;
+  if (dev < 64) known[dev] = n + 1;
+  return n;
 }
 
-// CTAs of a row.  A row's passes are bound by its SM where there are many rows (one CTA each, two an SM), by the cluster's
-// exchanges where there are few: with 1, 4, 8 CTAs a row 256 x 102400 bf16 takes 79 to 88, 93, 164 us, 32 x 102400 f32
-// 62 to 76, 35 to 38, 30 to 32, one row of 50257 24.8, 16.8, 16.4 (two draws of the settings).
+// C CTAs a row where a CTA's part is worth one and all rows run at once; *done tells whether it was launched
+template <typename In, bool RESIDENT, int C>
+cudaError_t launch_at_once(const SampleParams &p, int B, cudaStream_t st, bool *done) {
+  cudaError_t e;
+  if (B > clusters_at_once<In, RESIDENT, C>(&e) || e != cudaSuccess) return e;
+  *done = true;
+  Launch<In, RESIDENT, C> l(B, RESIDENT ? (p.chunk * sizeof(In) + 15) / 16 * 16 : 0, st);
+  return cudaLaunchKernelEx(&l.cfg, sample_kernel<In, RESIDENT, C>, p);
+}
+
+template <typename In, int C>
+cudaError_t try_row(SampleParams p, int B, cudaStream_t st, bool *done) {
+  if (*done || p.V <= C * 1024) return cudaSuccess;
+  p.chunk = ((p.V + C - 1) / C + 15) / 16 * 16;
+  return p.chunk * (int64_t)sizeof(In) <= kHeld ? launch_at_once<In, true, C>(p, B, st, done)
+                                                : launch_at_once<In, false, C>(p, B, st, done);
+}
+
+// CTAs of a row: as many as let every row run at once, up to 8.  A row's passes are bound by its SM, so more CTAs a row are
+// faster until clusters have to wait for one another, which the GPU's groups of SMs decide: 8 fit up to 33 or 34 rows, 4 up to
+// 70 or 71, 2 up to 148.  bf16 rows of 102400, top-k, with 1, 2, 4, 8 CTAs a row: 33 rows -, 29, 24, 24 us, 35 rows -, 30, 24, 38,
+// 70 rows -, 34, 27, 58, 72 rows -, 33, 41, 59, 148 rows 34, 36, 67, -; rows of mixed settings differ in length, so that there
+// 2 take 70 us at 148 rows where 1 takes 99.  Beyond, one CTA a row: 256 rows of top-p 82, 81, 95, 164.
 template <typename In>
 cudaError_t launch_row(SampleParams p, int B, cudaStream_t st) {
-  const int C = 8 * B <= 2 * 148 && p.V > 8 * 1024 ? 8 : B <= 148 && p.V > 4 * 1024 ? 4 : 1;
-  p.chunk = ((p.V + C - 1) / C + 15) / 16 * 16;
-  const bool held = p.chunk * (int64_t)sizeof(In) <= kHeld;
-  if (C == 1) return launch<In, false, 1>(p, B, st);
-  if (C == 4) return held ? launch<In, true, 4>(p, B, st) : launch<In, false, 4>(p, B, st);
-  return held ? launch<In, true, 8>(p, B, st) : launch<In, false, 8>(p, B, st);
+  bool done = false;
+  cudaError_t e = try_row<In, 8>(p, B, st, &done);
+  if (e == cudaSuccess) e = try_row<In, 4>(p, B, st, &done);
+  if (e == cudaSuccess) e = try_row<In, 2>(p, B, st, &done);
+  if (e != cudaSuccess || done) return e;
+  p.chunk = (p.V + 15) / 16 * 16;
+  Launch<In, false, 1> l(B, 0, st);
+  return cudaLaunchKernelEx(&l.cfg, sample_kernel<In, false, 1>, p);
 }
 
 }  // namespace
