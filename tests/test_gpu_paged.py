@@ -155,6 +155,69 @@ def test_append_matches_the_formulas(case, bits):
     assert c.status() == 0
 
 
+def _sum_squares_in_order(x):
+    """sum x^2 over the last dimension in f32, each step rounded: 256 dimensions first add their halves, 128 add up runs of 4
+    neighbours, and then what there is adds its halves until one is left."""
+    s = x * x
+    if s.shape[-1] == 256:
+        s = s[..., :128] + s[..., 128:]
+    if s.shape[-1] == 128:
+        r = s.unflatten(-1, (32, 4))
+        s = ((r[..., 0] + r[..., 1]) + r[..., 2]) + r[..., 3]
+    while s.shape[-1] > 1:
+        half = s.shape[-1] // 2
+        s = s[..., :half] + s[..., half:]
+    return s
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("hd,H,kv,rot,pairs", [(64, 6, 3, 64, False), (64, 4, 2, 32, True), (128, 6, 3, 128, False),
+                                               (128, 8, 2, 64, True), (256, 4, 2, 256, True), (256, 2, 1, 128, False)])
+def test_append_is_the_stated_order_to_the_bit(hd, H, kv, rot, pairs, f32, bits):
+    """Queries, codes, scales and minima equal, bit for bit, f32 arithmetic in the stated order with every step rounded on its
+    own: a key near a tie takes the same code in any call shape."""
+    import torch
+    rng = np.random.default_rng(hd + H + f32)
+    n, eps = 700, 1e-6
+    c = _cache([n], kv, hd, 64, bits, rng)
+    x = torch.from_numpy((2 * rng.standard_normal((n, (H + 2 * kv) * hd))).astype(np.float32)).cuda()
+    x = x if f32 else x.bfloat16()
+    g_q, g_k = (torch.from_numpy(rng.uniform(0.5, 1.5, hd).astype(np.float32)).cuda() for _ in range(2))
+    cos, sin = _tables(n, rot)
+    pos, seq = torch.arange(n, dtype=torch.int32).cuda(), torch.zeros(n, dtype=torch.int32).cuda()
+    q = c.append(x, pos, seq, H, cos=cos, sin=sin, pairs=pairs, g_q=g_q, g_k=g_k, eps=eps)
+
+    y = x.float().view(n, -1, hd)
+    out = []
+    for h, g in ((y[:, :H], g_q), (y[:, H:H + kv], g_k)):
+        h = h * torch.rsqrt(_sum_squares_in_order(h) * (1.0 / hd) + eps) * g
+        j = torch.arange(rot // 2, device="cuda")
+        a, b = (2 * j, 2 * j + 1) if pairs else (j, j + rot // 2)
+        u, w, cc, ss = h[..., a], h[..., b], cos[:, None], sin[:, None]
+        r = h.clone()
+        r[..., a], r[..., b] = u * cc - w * ss, w * cc + u * ss
+        out.append(r)
+    assert torch.equal(q.view(n, H, hd).view(torch.int16), out[0].bfloat16().view(torch.int16))
+    kvs = torch.stack((out[1], y[:, H + kv:]), 2)   # [n, kv, 2, hd]
+    page = c.table[0, (pos // 64).long()].long()
+    pool = c.pool[page].view(n, kv, 2, -1)
+    row = (pos % 64).long()
+    if bits == 16:
+        got = pool.view(n, kv, 2, 64, hd * 2)[torch.arange(n), :, :, row]
+        assert torch.equal(got.contiguous().view(torch.int16), kvs.bfloat16().view(torch.int16))
+        return
+    codes = pool[..., :64 * hd // 2].reshape(n, kv, 2, 64, hd // 2)[torch.arange(n), :, :, row]
+    marks = pool[..., 64 * hd // 2:].reshape(n, kv, 2, 64, hd // GROUP * 4)[torch.arange(n), :, :, row]
+    grp = kvs.unflatten(-1, (-1, GROUP))
+    mn, mx = grp.amin(-1), grp.amax(-1)
+    third = torch.tensor(1.0, device="cuda") / 15
+    scale, least = ((mx - mn) * third).bfloat16(), mn.bfloat16()
+    assert torch.equal(marks.contiguous().view(torch.int16), torch.stack((scale, least), -1).flatten(-2).view(torch.int16))
+    code = torch.round((grp - least.float()[..., None]) / scale.float()[..., None]).clamp(0, 15).to(torch.uint8).flatten(-2)
+    assert torch.equal(codes, code[..., 0::2] | code[..., 1::2] << 4)
+
+
 def test_append_skips_rows_outside_the_cache_and_keeps_nan_visible():
     import torch
     from thvm_b200 import _lib as L
