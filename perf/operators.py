@@ -155,7 +155,9 @@ def prepare(case, seed):
         B, V, kind = case["rows"], case["vocab"], case["kind"]
         x = 2 * torch.randn(B, V, generator=g, device=dev)
         at = torch.randint(V, (B, 24), generator=g, device=dev)
-        x.scatter_(1, at, 5 + 9 * torch.rand(B, 24, generator=g, device=dev))  # the few tokens that a model holds likely
+        likely = 5 + 9 * torch.rand(B, 24, generator=g, device=dev)  # the few tokens that a model holds likely
+        for a, v in zip(at.split(1, 1), likely.split(1, 1)):  # one after the other: an id that comes twice keeps its last value
+            x.scatter_(1, a, v)
         if case["masked"]:
             x.masked_fill_(torch.rand(B, V, generator=g, device=dev) < 0.3, -math.inf)
         s["logits"] = x.to(torch.bfloat16) if case["bf16"] else x
