@@ -541,3 +541,66 @@ def test_refusals():
     assert L.lib().sm100_paged_attention(c._desc, ctypes.byref(small), None) == L.ERR_ARG
     assert b"scratch" in L.lib().sm100_last_error()
     assert c.status() == 0
+
+
+def test_long_sums_of_codes_do_not_lean():
+    """65536 tokens a sequence whose values cancel in pairs, equal weights (q = 0): the output is zero.
+
+    A value is m + c s with s = 205 / 1024, m = -7.5 s rounded to bf16, codes c and 15 - c in turn: a pair's sum is
+    2 m + 15 s, the rounding of m that is left.  The formula's output is m + 7.5 s, below 2^-9 of |v|'s mean.  Weights are
+    1 and their products with s exact, so what is left is the f32 sums' rounding: of terms whose running sum stays
+    within a tile's, 2^-17 of the mean |v| is ample; sums of 16384 offset codes that are rounded towards zero
+    lean by 2^-13 of it.  Sequences share 16 pages, so that each warp's sums are long and the pool small."""
+    import torch
+    from thvm_b200.paged import PagedCache
+    rng = np.random.default_rng(21)
+    n_seq, kv, hd, page, n = 64, 8, 128, 64, 65536
+    c = PagedCache.empty(n_seq, n // page, 16, kv, hd, page, 4)
+    c.table.copy_(torch.from_numpy(rng.permuted(np.tile(np.arange(16, dtype=np.int32), (n_seq, n // page // 16)), axis=1)))
+    x = c.pool.view(16, kv, 2, -1)
+    code = torch.from_numpy(rng.integers(0, 16, (16, kv, 2, page // 2, hd)).astype(np.uint8)).cuda()
+    code = torch.stack((code, 15 - code), 4).flatten(3, 4)   # tokens 2 i and 2 i + 1
+    x[..., :page * hd // 2] = (code[..., 0::2] | code[..., 1::2] << 4).flatten(3)
+    s = torch.tensor(205 / 1024).bfloat16()
+    m = (-7.5 * s.float()).bfloat16()
+    x[..., page * hd // 2:] = torch.stack((s, m)).cuda().view(torch.uint8).repeat(page * hd // GROUP)
+    for H in (8, 64):   # both forms of the products: up to 4 query columns, and 8
+        q = torch.zeros(n_seq, H, hd, dtype=torch.bfloat16, device="cuda")
+        got = c.attend(q, torch.full((n_seq,), n, dtype=torch.int32).cuda()).double()
+        want = float(m) + 7.5 * float(s)
+        assert float((got - want).abs().max()) <= 2.0 ** -8 * abs(want) + 2.0 ** -17 * 4 * float(s)
+    assert c.status() == 0
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("H", [1, 4, 8])
+def test_weights_keep_sixteen_bits(bits, H):
+    """Values +-a whose weighted sum nearly cancels, so that the output's own rounding is small and the weights' shows.
+
+    A weight enters as two bf16 parts: off by at most 2^-8 of 2^-8 of it; its logit's f32 error (below 16) and 2^x add
+    2^-18, the sums of 32 tokens 2^-19: 2^-15 of sum p |v| holds all.  Weights of 8 bits are off by 2^-9 of the root of
+    sum p^2, some 2^-11."""
+    import torch
+    rng = np.random.default_rng(31 + bits + H)
+    n, hd = 32, 64
+    c = _cache([n], 1, hd, 16, bits, rng)
+    x = torch.from_numpy(rng.standard_normal((n, 3 * hd)).astype(np.float32)).cuda()
+    q = torch.from_numpy(rng.standard_normal((1, H, hd)).astype(np.float32)).cuda().bfloat16()
+    q[:] = q[:, :1]
+    pos, seq = torch.arange(n).int().cuda(), torch.zeros(n).int().cuda()
+    c.append(x, pos, seq, 1)
+    k = _unpack(c)[0][c.table[0, pos.long() // 16].long(), 0, 0, pos.long() % 16]
+    p = torch.softmax(k @ q[0, 0].double() * hd ** -0.5, 0).cpu().numpy()
+    sign, left = np.zeros(n), 0.0
+    for i in np.argsort(-p):      # the largest first, each against what is left
+        sign[i] = -1.0 if left > 0 else 1.0
+        left += sign[i] * p[i]
+    a = 7.5 * 0.25                # codes 0 and 15, scale 1 / 4
+    along = torch.from_numpy(rng.choice([-1.0, 1.0], hd)).float()
+    along[:2] = torch.tensor([1.0, -1.0])
+    x[:, 2 * hd:] = (a * torch.from_numpy(sign).float()[:, None] * along).cuda()
+    c.append(x, pos, seq, 1)
+    want, size = _attend_want(c, q, [n], [1], hd ** -0.5)
+    assert float(want.abs().max()) <= 0.02 * a   # they do cancel
+    err = (c.attend(q, torch.tensor([n], dtype=torch.int32).cuda()).double() - want).abs()
+    assert bool((err <= 2.0 ** -8 * want.abs() + 2.0 ** -15 * size).all()), float((err / size).max())

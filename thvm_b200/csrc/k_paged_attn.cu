@@ -36,11 +36,16 @@
 // loads in bf16, whole code words in 4 bits.  (tcgen05 would want 128 rows of
 // queries, and unpacked codes written back to shared memory.)
 //
-// 4 bits: a code c enters the products as an exact bf16 integer (128 + c in
-// K, 16 + c in V, each put together by a shift and one AND-OR; the offset of V
-// is the smaller one since its sums cancel).  A group's scale and minimum are
-// applied outside: S = s * (Q . (128 + c)) + (m - 128 s) * sum Q per group of 64
-// dimensions, and p * s per token is V's weight, sum p (m - 16 s) its shift.
+// 4 bits: a code c enters the products as an exact bf16 integer (128 + c in K;
+// in V 16 + c for tokens 0 .. 7 of 16 and c - 31 = -(16 + (15 - c)) for the
+// others), put together by a shift and one three-input logic operation, a known
+// way to make numbers of codes.  A group's scale and minimum are applied outside:
+// S = s * (Q . (128 + c)) + (m - 128 s) * sum Q per group of 64 dimensions, and
+// p * s per token is V's weight, sum p (m - 16 s) or p (m + 31 s) its shift.  The
+// products round their running sums towards zero: with one sign for all tokens
+// the sums of 16 + c grew to some 20 times the output, and long ones leaned by
+// 2^-13 of the mean |v|; with two signs they stay near zero (64 x up to 16384: 17 % of
+// the outputs were a bf16 step off the rounded result, 1.4 % are, in the same time).
 // Weights enter as bf16 hi + lo, so their rounding (2^-17) is far below the
 // output's; with up to 4 query columns the low parts are columns 4 to 7 of the
 // same product.
@@ -128,18 +133,27 @@ __device__ __forceinline__ uint32_t split_columns(float w0, float w1, bool low) 
   return transpose8x8(low ? l : h);
 }
 
-// (x & mask) | bits as the one instruction that it is (written plainly it became two, a third of a step's instructions)
+// (x & mask) | bits as the one instruction that it is (written plainly it became two, a third of a step's instructions),
+// and (~x & mask) | bits
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
   return r;
 }
+__device__ __forceinline__ uint32_t nand_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xae;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
+  return r;
+}
 
 // two codes of a word (bits 4 i and 4 i + 16) as bf16 128 + c
 __device__ __forceinline__ uint32_t codes128(uint32_t w, int i) { return and_or(w >> (4 * i), 0x000f000fu, 0x43004300u); }
-// the same as bf16 16 + c (the code in the upper four bits of the mantissa)
+// the same as bf16 16 + c (the code in the upper four bits of the mantissa), and as c - 31 = -(16 + (15 - c))
 __device__ __forceinline__ uint32_t codes16(uint32_t w, int i) {
   return and_or(i == 0 ? w << 3 : w >> (4 * i - 3), 0x00780078u, 0x41804180u);
+}
+__device__ __forceinline__ uint32_t codes31(uint32_t w, int i) {
+  return nand_or(i == 0 ? w << 3 : w >> (4 * i - 3), 0x00780078u, 0xc180c180u);
 }
 
 // The line: units in the order (sequence, key head, column tile), each kPad
@@ -526,7 +540,7 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
               const uint32_t wc = *reinterpret_cast<const uint32_t *>(vc + 8 * ROW);
               const uint32_t wd = *reinterpret_cast<const uint32_t *>(vc + 9 * ROW);
               const float s0 = bf16_lo(m0), s8 = bf16_lo(m8);
-              const float b0 = fmaf(-16.0f, s0, bf16_hi(m0)), b8 = fmaf(-16.0f, s8, bf16_hi(m8));
+              const float b0 = fmaf(-16.0f, s0, bf16_hi(m0)), b8 = fmaf(31.0f, s8, bf16_hi(m8));
               uint32_t p0, p8, r0, r8;
               float w[4];
               if (!edge) {
@@ -556,8 +570,8 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
 #pragma unroll
               for (int j = 0; j < 4; j++) {   // dimensions 8 g + 2 j, 8 g + 2 j + 1 of the group
                 const int i = 2 * (j & 1);
-                const uint32_t af[4] = {codes16(lo[j >> 1], i), codes16(lo[j >> 1], i + 1), codes16(hi[j >> 1], i),
-                                        codes16(hi[j >> 1], i + 1)};
+                const uint32_t af[4] = {codes16(lo[j >> 1], i), codes16(lo[j >> 1], i + 1), codes31(hi[j >> 1], i),
+                                        codes31(hi[j >> 1], i + 1)};
                 mma_bf16(o[4 * gr + j], af, p0, p8);
                 if constexpr (!DUAL) mma_bf16(o[4 * gr + j], af, r0, r8);
               }
