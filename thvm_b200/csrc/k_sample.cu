@@ -37,6 +37,7 @@
 // there on sums are 64-bit integers in units of 2^-40, so no order of arrival
 // enters a result.
 #include "common.cuh"
+#include "sample_bins.h"
 
 #include <cooperative_groups.h>
 #include <float.h>
@@ -95,6 +96,9 @@ __device__ __forceinline__ int id_of(uint64_t pl) { return (int)~(uint32_t)pl; }
 
 // A weight, or a thread's sum of some, in units of 2^-40
 __device__ __forceinline__ uint64_t fixed(float w) { return __float2ull_rn(w * 1099511627776.0f); }
+
+// The estimated weight of a bin's ids
+__device__ __forceinline__ BinSum bin_weight(int bin, uint32_t ids) { return ids * fixed(__expf(-(float)bin / kPerNat)); }
 
 __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
@@ -155,8 +159,8 @@ struct alignas(16) Shared {
   struct {
     uint64_t top, row, near, above, best, kept;   // largest place; weight of all ids, of those in the bins; measure above the
                                                   // list's bins; winner there and kept weight
+    BinSum heavy;                                 // the slice's estimated weight
     uint32_t ids, n_list;                         // ids in its slice of bins; places on its list
-    float heavy;                                  // the slice's estimated weight
   } from[kMost];
   uint64_t cut, sum, over;         // from CTA 0
   uint32_t done, missed;
@@ -430,7 +434,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   constexpr int kB = kBins / C / kThreads;   // a CTA's slice of the bins, kB neighbours a thread
   const int bin0 = (rank * kThreads + tid) * kB;
   uint32_t cnt[kB], c_before = 0, valid = 0;
-  float w_before = 0.0f, unseen = 0.0f;   // unseen: the bins' weight beyond their estimate
+  BinSum w_before = 0;
+  float unseen = 0.0f;   // the bins' weight beyond their estimate
   float l_far = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kB; i++) cnt[i] = 0;
@@ -480,25 +485,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     if (by_weight) {
       total = cluster_sum(peer->row);
       near = cluster_sum(peer->near);
-      unseen = (float)near * 0x1p-40f;
     }
     uint32_t ids = 0;
-    float heavy = 0.0f;
+    BinSum heavy = 0;
 #pragma unroll
-    for (int i = 0; i < kB; i++) ids += cnt[i], heavy += cnt[i] * __expf(-(float)(bin0 + i) / kPerNat);
+    for (int i = 0; i < kB; i++) ids += cnt[i], heavy += bin_weight(bin0 + i, cnt[i]);
     c_before = block_before(ids, reinterpret_cast<uint32_t *>(sh.red), &ids);
-    w_before = block_before(heavy, reinterpret_cast<float *>(sh.red2), &heavy);
+    w_before = block_before(heavy, sh.red2, &heavy);
     if (to) to->from[rank].ids = ids, to->from[rank].heavy = heavy;
     sync();
     const uint32_t c = (tid & 31) < C ? peer->ids : 0;
-    const float h = (tid & 31) < C ? peer->heavy : 0.0f;
+    const BinSum h = (tid & 31) < C ? peer->heavy : 0;
+    BinSum all = 0;
 #pragma unroll
     for (int r = 0; r < C; r++) {
       const uint32_t cr = __shfl_sync(0xffffffffu, c, r);
-      const float hr = __shfl_sync(0xffffffffu, h, r);
+      const BinSum hr = __shfl_sync(0xffffffffu, h, r);
       if (r < rank) c_before += cr, w_before += hr;
-      valid += cr, unseen -= hr;
+      valid += cr, all += hr;
     }
+    unseen = (float)(int64_t)(near - all) * 0x1p-40f;
     last_bin = sc.bin(l_far);
     if (by_weight && !by_count && (double)near < (double)p * (double)total) past = true;   // top-p cuts nothing that min-p leaves
     if (by_count && (uint32_t)k >= valid) by_count = false;   // top-k leaves every id there is
@@ -520,25 +526,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       if (filtered) {
         {
           const float spread = weigh ? 1.0f : 0.0f;
-          const float goals[kGoals] = {goal * (1.0f - 0.0045f * spread), goal * (1.0f + 0.0045f * spread),
-                                       guess * (1.0f - 0.001f * spread), guess * (1.0f + 0.001f * spread),
-                                       guess * (1.0f - 0.0002f * spread), guess * (1.0f + 0.0002f * spread), guess};
+          const auto sum_of = [&](float v) { return (BinSum)fmaxf(weigh ? v * 0x1p40f : v, 0.0f); };
+          const BinSum goals[kGoals] = {sum_of(goal * (1.0f - 0.0045f * spread)), sum_of(goal * (1.0f + 0.0045f * spread)),
+                                        sum_of(guess * (1.0f - 0.001f * spread)), sum_of(guess * (1.0f + 0.001f * spread)),
+                                        sum_of(guess * (1.0f - 0.0002f * spread)), sum_of(guess * (1.0f + 0.0002f * spread)),
+                                        sum_of(guess)};
           const auto tell = [&](int g, const Crossing &x) {
             for (int r = 0; r < C; r++) (C > 1 ? cluster.map_shared_rank(&sh, r) : &sh)->cross[g] = x;
           };
           uint32_t cc = c_before;
-          float ww = w_before;
+          BinSum ww = w_before;
 #pragma unroll
           for (int i = 0; i < kB; i++) {
-            if (bin0 + i == last_bin) tell(kLast, Crossing{last_bin, cc, cc + cnt[i], ww});
+            if (bin0 + i == last_bin) tell(kLast, Crossing{last_bin, cc, cc + cnt[i], (float)ww * 0x1p-40f});
             if (cnt[i] == 0 || bin0 + i > last_bin) continue;
             const uint32_t c1 = cc + cnt[i];
-            const float w1 = ww + cnt[i] * __expf(-(float)(bin0 + i) / kPerNat);
+            const BinSum w1 = ww + bin_weight(bin0 + i, cnt[i]);
 #pragma unroll
-            for (int g = 0; g < kGoals; g++) {
-              const float was = weigh ? ww : (float)cc, now = weigh ? w1 : (float)c1;
-              if (now >= goals[g] && (was < goals[g] || cc == 0)) tell(g, Crossing{bin0 + i, cc, c1, ww});
-            }
+            for (int g = 0; g < kGoals; g++)   // one thread of the cluster owns a goal
+              if (reaches<BinSum>(weigh ? ww : cc, weigh ? w1 : c1, cc == 0, goals[g]))
+                tell(g, Crossing{bin0 + i, cc, c1, (float)ww * 0x1p-40f});
             cc = c1, ww = w1;
           }
         }
