@@ -92,3 +92,31 @@ def test_sample_refusals():
         assert _sample(**bad) == L.ERR_ARG, bad
     assert _sample(dtype=L.DT_I32) == L.ERR_UNSUPPORTED
     assert _sample(B=0) == L.OK
+
+
+def test_scratch_keeps_what_a_graph_may_hold(monkeypatch):
+    import pytest
+    import torch
+    from thvm_b200.paged import Scratch
+    cpu, capturing = torch.device("cpu"), []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: bool(capturing))
+    s = Scratch()
+    small = s.take(64, cpu).ptr
+    assert s.take(32, cpu).ptr == s.take(64, cpu).ptr == small   # large enough: it stays where it is
+    assert s.take(128, cpu).ptr != small and s.nbytes == 128
+    assert [b.data_ptr() for b in s.held] == [small, s.ptr]      # the earlier memory is no one else's
+    with pytest.raises(ValueError):
+        s.take(16, torch.device("cuda", 0))
+    capturing.append(True)
+    assert s.take(128, cpu).nbytes == 128
+    with pytest.raises(RuntimeError):
+        s.take(129, cpu)
+
+
+def test_widest_workspace_is_that_of_eight_columns():
+    f = L.lib().sm100_paged_attention_ws_bytes
+    for bits in (4, 16):
+        for hd in (64, 128, 256):
+            c = _cache(bits=bits, head_dim=hd)
+            most = f(ctypes.byref(c), 2, 8)
+            assert all(f(ctypes.byref(c), 2 * g, r) <= most for g in (1, 2, 5, 64) for r in (1, 2, 7, 4096))

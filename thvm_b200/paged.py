@@ -23,16 +23,22 @@ _addressof = ctypes.addressof
 
 
 class Scratch:
-    """The attention's workspace: grows to what its calls need."""
+    """The attention's workspace.  A cache takes what its widest call needs when
+    it is made, so no call moves it; where a cache of wider heads joins later,
+    the earlier memory is kept, since a captured graph may hold its address."""
 
     def __init__(self):
-        self.buf, self.ptr, self.nbytes = None, 0, 0
+        self.held, self.ptr, self.nbytes = [], 0, 0
 
     def take(self, nbytes: int, device):
+        import torch
+        if self.held and self.held[-1].device != device:
+            raise ValueError(f"a scratch on {self.held[-1].device} for a cache on {device}")
         if nbytes > self.nbytes:
-            import torch
-            self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)   # counters start at zero
-            self.ptr, self.nbytes = self.buf.data_ptr(), nbytes
+            if torch.cuda.is_current_stream_capturing():   # the zeros would be written by the replays alone
+                raise RuntimeError("the attention's workspace cannot be made while a graph is captured")
+            self.held.append(torch.zeros(nbytes, dtype=torch.uint8, device=device))   # counters start at zero
+            self.ptr, self.nbytes = self.held[-1].data_ptr(), nbytes
         return self
 
 
@@ -63,6 +69,8 @@ class PagedCache:
         self._append, self._read, self._attention = (
             self.lib.sm100_paged_append, self.lib.sm100_paged_read, self.lib.sm100_paged_attention)
         self._need: dict[tuple[int, int], int] = {}
+        # 8 query columns a unit are the widest layout
+        self.scratch.take(int(self.lib.sm100_paged_attention_ws_bytes(self._desc, self.kv_heads, 8)), pool.device)
 
     @classmethod
     def empty(cls, n_seq: int, max_pages: int, n_pages: int, kv_heads: int, head_dim: int, page: int = 32,
@@ -158,8 +166,6 @@ class PagedCache:
                 raise ValueError(f"heads {heads} (a multiple of {self.kv_heads}), max_rows {max_rows}")
             self._need[heads, max_rows] = need
         ws = self.scratch
-        if need > ws.nbytes:
-            ws.take(need, self._device)
         a = L.Sm100PagedAttnArgs(q.data_ptr(), dense("kv_len", kv_len, i32, self._n_seq),
                                  None if q_off is None else dense("q_off", q_off, i32, self._n_seq + 1), out_ptr,
                                  ws.ptr, ws.nbytes, step if T > 1 else 0, T, heads, max_rows,
