@@ -768,7 +768,8 @@ int sm100_paged_read(const Sm100PagedCache *c, const int32_t *pos, const int32_t
  * rows q_off[s] .. q_off[s + 1] - 1 (q_off NULL: row s alone, T = n_seq), at
  * most max_rows of them, at its last positions: of n rows, row r sees keys
  * 0 .. kv_len[s] - n + r (kv_len counts the new tokens, appended before).  A
- * row that sees none (an idle sequence: kv_len 0) is zeros.  Tokens whose page
+ * row that sees none (an idle sequence: kv_len 0), or only scores of -inf, is
+ * zeros; a score of NaN or +inf makes the row's head NaN.  Tokens whose page
  * is outside the pool are left out and set the status word, as does a length
  * past max_pages * page (cut there).  scale >= 0.  q bf16, row stride ld_q elements (0:
  * dense), a multiple of 8; q, out, ws 16-byte aligned; heads / kv_heads whole.

@@ -637,3 +637,53 @@ def test_graph_stays_right_after_wider_eager_calls():
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             type(c)(c.pool, c.table, page, hd, 4)
     assert c.status() == 0
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("hd,H,kv", [(64, 4, 2), (128, 16, 2), (256, 2, 2)])
+def test_nan_scores_reach_their_rows(bits, hd, H, kv):
+    """A key with a NaN, alone in its warp, tile or CTA or not: every row and head that sees it is NaN, the other key head's
+    are the formula's.  A NaN in a query makes its head NaN, and no other."""
+    import torch
+    rng = np.random.default_rng(hd + bits)
+    G = H // kv
+    for n, at in ((1, 0), (17, 16), (33, 32), (65, 64), (129, 128), (200, 0), (6000, 0), (6000, 3011), (6000, 5999)):
+        c = _cache([n], kv, hd, 16, bits, rng)
+        _fill(c, [n], rng)
+        q = torch.from_numpy(rng.standard_normal((1, H, hd)).astype(np.float32)).cuda().bfloat16()
+        kv_len = torch.tensor([n], dtype=torch.int32).cuda()
+        want, size = _attend_want(c, q, [n], [1], hd ** -0.5)
+        broken = q.clone()
+        broken[0, 1, 5] = float("nan")
+        got = c.attend(broken, kv_len)
+        assert bool(torch.isnan(got[0, 1]).all()), n
+        rest = [h for h in range(H) if h != 1]
+        _check_attention(got[:, rest], want[:, rest], size[:, rest])
+        k, v = c.read(torch.tensor([at], dtype=torch.int32).cuda(), torch.zeros(1, dtype=torch.int32).cuda())
+        x = torch.cat((torch.zeros(kv * hd).cuda(), k.flatten().float(), v.flatten().float()))[None]
+        x[0, kv * hd + 3] = float("nan")   # key head 0
+        c.append(x, torch.tensor([at], dtype=torch.int32).cuda(), torch.zeros(1, dtype=torch.int32).cuda(), kv)
+        got = c.attend(q, kv_len)
+        assert bool(torch.isnan(got[0, :G]).all()), (n, at)
+        want, size = _attend_want(c, q, [n], [1], hd ** -0.5)   # (4 bits: the values were put in once more)
+        _check_attention(got[:, G:], want[:, G:], size[:, G:])
+        assert c.status() == 0
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_nan_scores_of_later_tokens_stay_out(bits):
+    """Verify rows: the rows before a NaN key are the formula's, the others NaN, also where the key is a tile's first."""
+    import torch
+    rng = np.random.default_rng(bits)
+    for n in (66, 130, 260):
+        c = _cache([n], 1, 128, 64, bits, rng)
+        _fill(c, [n], rng)
+        q = torch.from_numpy(rng.standard_normal((4, 4, 128)).astype(np.float32)).cuda().bfloat16()
+        want, size = _attend_want(c, q, [n], [4], 128 ** -0.5)
+        x = torch.zeros(1, 3 * 128).cuda()
+        x[0, 128] = float("nan")
+        c.append(x, torch.tensor([n - 2], dtype=torch.int32).cuda(), torch.zeros(1, dtype=torch.int32).cuda(), 1)
+        got = c.attend(q, torch.tensor([n], dtype=torch.int32).cuda(), q_off=torch.tensor([0, 4], dtype=torch.int32).cuda(),
+                       max_rows=4)
+        _check_attention(got[:2], want[:2], size[:2])
+        assert bool(torch.isnan(got[2:]).all())

@@ -630,7 +630,8 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
       if (lane == 0) mbar_arrive(&empty[st]);
     }
 
-    // ---- the warps' parts of the unit joined
+    // ---- the warps' parts of the unit joined.  A maximum of -inf: no token that counts, a sum of 0, or none but scores of
+    // NaN (which a maximum passes over), a sum of NaN: the sum then stands for the part's weight
     const bool mine = !DUAL || cq < 2;   // this thread's columns are query columns
 #pragma unroll
     for (int e = 0; e < 2; e++) {
@@ -654,8 +655,8 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
 #pragma unroll
       for (int i = 0; i < NW; i++) top = fmaxf(top, wm[i][col]);
 #pragma unroll
-      for (int i = 0; i < NW; i++) sum += wm[i][col] == -INFINITY ? 0.0f : wl[i][col] * ex2(wm[i][col] - top);
-      f[e] = m[e] == -INFINITY ? 0.0f : ex2(m[e] - top);
+      for (int i = 0; i < NW; i++) sum += wm[i][col] == -INFINITY ? wl[i][col] : wl[i][col] * ex2(wm[i][col] - top);
+      f[e] = m[e] == -INFINITY ? l[e] : ex2(m[e] - top);
       if (warp == 0 && g == 0 && mine) um[col] = top, ul[col] = sum;
     }
     // where the piece ends inside the unit, or began inside it: a part
@@ -729,13 +730,16 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
         for (int x = c0 + lane; x <= c1; x += 32) {
           const float *p = part_of(x) + S::ACC * 128 + col;
           const float pm = __ldcg(p), pl = __ldcg(p + COLS);
-          if (pm == -INFINITY) continue;
+          if (pm == -INFINITY) {
+            sum += pl;
+            continue;
+          }
           const float v = fmaxf(top, pm);
           sum = sum * ex2(top - v) + pl * ex2(pm - v);
           top = v;
         }
         const float all = warp_max(top);
-        sum = warp_sum(top == -INFINITY ? 0.0f : sum * ex2(top - all));
+        sum = warp_sum(top == -INFINITY ? sum : sum * ex2(top - all));
         if (lane == 0) um[col] = all, ul[col] = sum;
       }
 #pragma unroll
@@ -751,7 +755,7 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
         sync();
         for (int i = tid; i < n * COLS; i += NW * 32) {
           const float pm = __ldcg(part_of(x0 + i / COLS) + S::ACC * 128 + i % COLS);
-          weights[i] = pm == -INFINITY ? 0.0f : ex2(pm - um[i % COLS]);
+          weights[i] = pm == -INFINITY ? 0.0f : ex2(pm - um[i % COLS]);   // (a sum of NaN is in the unit's)
         }
         sync();
         // a warp's parts, UN of them under way at a time; with 4 columns the idle half of the lanes takes every other one
