@@ -687,3 +687,22 @@ def test_nan_scores_of_later_tokens_stay_out(bits):
                        max_rows=4)
         _check_attention(got[:2], want[:2], size[:2])
         assert bool(torch.isnan(got[2:]).all())
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("scale", [0.0, 1e-42, 1e-30])
+def test_scale_zero_is_the_mean(bits, scale):
+    """With a scale of nothing a row is the mean of the values that it sees, for lengths that end inside a tile, later tokens
+    of other rows, idle sequences and units cut between CTAs."""
+    import torch
+    rng = np.random.default_rng(bits)
+    for lens, rows in (([1, 17, 33, 0, 130, 64], [1] * 6), ([40, 3, 100], [5, 7, 4]), ([5001], [1]), ([90], [33])):
+        c = _cache(lens, 2, 64, 16, bits, rng)
+        _fill(c, lens, rng)
+        q = torch.from_numpy(rng.standard_normal((sum(rows), 4, 64)).astype(np.float32)).cuda().bfloat16()
+        q_off = torch.tensor(np.concatenate([[0], np.cumsum(rows)]), dtype=torch.int32).cuda()
+        want, size = _attend_want(c, q, lens, rows, scale)
+        got = c.attend(q, torch.tensor(lens, dtype=torch.int32).cuda(), q_off=q_off, max_rows=max(rows), scale=scale)
+        assert bool(torch.isfinite(got).all())
+        _check_attention(got, want, size)
+        assert c.status() == 0

@@ -120,3 +120,7 @@ def test_widest_workspace_is_that_of_eight_columns():
             c = _cache(bits=bits, head_dim=hd)
             most = f(ctypes.byref(c), 2, 8)
             assert all(f(ctypes.byref(c), 2 * g, r) <= most for g in (1, 2, 5, 64) for r in (1, 2, 7, 4096))
+
+
+def test_attention_refuses_a_scale_whose_logarithm_base_overflows():
+    assert _attend(_cache(), scale=3e38) == L.ERR_ARG

@@ -49,6 +49,8 @@
 // Weights enter as bf16 hi + lo, so their rounding (2^-17) is far below the
 // output's; with up to 4 query columns the low parts are columns 4 to 7 of the
 // same product.
+#include <float.h>
+
 #include "paged.cuh"
 #include "tma.cuh"
 
@@ -855,12 +857,15 @@ extern "C" int sm100_paged_attention(const Sm100PagedCache *c, const Sm100PagedA
   if (a->ws_bytes < need)
     return sm100_set_error(SM100_ERR_ARG, "paged_attention: %llu bytes of scratch, %llu needed",
                            (unsigned long long)a->ws_bytes, (unsigned long long)need);
-  if (!(a->scale >= 0.0f && a->scale <= 3e38f))
-    return sm100_set_error(SM100_ERR_ARG, "paged_attention: scale %g (0 or more, finite)", (double)a->scale);
+  if (!(a->scale >= 0.0f && a->scale <= 2e38f))   // times log2(e) it is finite
+    return sm100_set_error(SM100_ERR_ARG, "paged_attention: scale %g (0 to 2e38)", (double)a->scale);
   if ((int64_t)a->T * a->heads / c->kv_heads > INT32_MAX)
     return sm100_set_error(SM100_ERR_ARG, "paged_attention: %d rows in one call", a->T);
   AttnParams p{static_cast<const __nv_bfloat16 *>(a->q), a->kv_len, a->q_off, static_cast<__nv_bfloat16 *>(a->out),
-               nullptr, nullptr, ld, a->T, a->heads, a->heads / c->kv_heads, a->scale * 1.4426950408889634f};
+               nullptr, nullptr, ld, a->T, a->heads, a->heads / c->kv_heads,
+               // a hidden token's score is -inf before it is scaled, and -inf * 0 is NaN: a scale of 0 goes in as the smallest
+               // normal number, with which scores below 2^100 come out as 0 to f32's last bit
+               fmaxf(a->scale * 1.4426950408889634f, FLT_MIN)};
   cudaStream_t st = (cudaStream_t)stream;
   const bool q4 = c->bits == SM100_KV_Q4;
   if (c->head_dim == 64) return q4 ? launch_columns<64, 4>(v, p, a, st) : launch_columns<64, 16>(v, p, a, st);
