@@ -800,9 +800,10 @@ uint32_t sm100_paged_status(void);
  * id with the largest d_i - ln(noise_i) (equal ones: the lowest id): with
  * noise (f32 [B][V], row stride ld_noise) drawn from the unit exponential
  * distribution an id is chosen with probability w_i / (the kept weight), whose
- * logarithm is logp[b] (f32, or NULL).  temperature[b] <= 0 takes the first id
- * (logp 0).  Logits of -inf or NaN are left out, +inf counts as the largest
- * float; a row with none left gives id -1 and logp -inf.  temperature, top_k,
+ * logarithm is logp[b] (f32, or NULL).  temperature[b] or top_p[b] <= 0, min_p[b]
+ * > 1, or NaN in one of them takes the first id (logp 0).  Logits of -inf or NaN
+ * are left out, +inf counts as the largest float; a row with none left gives id
+ * -1 and logp -inf.  temperature, top_k,
  * top_p, min_p: device arrays [B], or NULL (1, all, all, all).  V < 2^23.  The
  * weights of the filters are summed exactly in units of 2^-40: the cut does
  * not depend on an order of summation. */

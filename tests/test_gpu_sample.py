@@ -304,3 +304,28 @@ def test_refusals():
         s(x[:, :0], n[:, :0])
     tok, logp = s(x[:0], n[:0])
     assert tok.numel() == 0 and logp.numel() == 0
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("V", [6, 1000, 40001])
+def test_no_top_p_leaves_the_first_id(V, bf16):
+    """top_p of 0, below it or NaN: the first id alone, whatever the other filters leave and however many ids tie with it;
+    NaN in temperature or min_p does the same."""
+    import torch
+    nan = math.nan
+    rng = np.random.default_rng(V)
+    g = torch.Generator("cuda")
+    g.manual_seed(V)
+    x = torch.zeros(3, V)
+    x[0, rng.permutation(V)[:max(1, V // 5)]] = 2.0   # many equal largest logits above equal ones
+    x[1] = torch.from_numpy(_levels(V, rng, 40))
+    x[2] = torch.from_numpy(rng.standard_normal(V).astype(np.float32))
+    x = (x.bfloat16() if bf16 else x).cuda()
+    want = [int(np.flatnonzero(r == r.max())[0]) for r in x.float().cpu().numpy()]
+    for _ in range(4):
+        noise = torch.empty(3, V, device="cuda").exponential_(generator=g)
+        for f in (dict(p=0.0), dict(p=-1.0), dict(p=nan), dict(k=300, p=0.0), dict(k=300, p=-0.5), dict(k=300, p=nan),
+                  dict(k=2, p=0.0), dict(k=700, p=0.0, m=0.01), dict(p=nan, m=0.5), dict(p=1e-45), dict(k=300, p=1e-45),
+                  dict(m=nan), dict(k=300, m=nan), dict(T=nan), dict(T=nan, p=0.9)):
+            tok, logp = _run(x, noise, **f)
+            assert tok.tolist() == want and logp.tolist() == [0.0] * 3, (f, tok.tolist(), want)

@@ -376,8 +376,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     return __shfl_sync(0xffffffffu, v, 0);
   };
   top = cluster_max(peer->top);
-  const float min_p = a.min_p ? a.min_p[b] : 0.0f;
-  if (top == 0 || !(T > 0.0f) || !(min_p <= 1.0f)) {   // nothing, or the first id alone
+  const float min_p = a.min_p ? a.min_p[b] : 0.0f, p = a.top_p ? a.top_p[b] : 1.0f;
+  if (top == 0 || !(T > 0.0f) || !(p > 0.0f) || !(min_p <= 1.0f)) {   // nothing, or the first id alone
     if (rank == 0 && tid == 0) {
       a.tok[b] = top == 0 ? -1 : id_of(top);
       if (a.logp) a.logp[b] = top == 0 ? -INFINITY : 0.0f;
@@ -387,7 +387,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   Scale sc;
   sc.set(logit_of(top), T);
   const bool wild = sc.lmax == FLT_MAX;   // there may be +inf among the logits
-  const float p = a.top_p ? a.top_p[b] : 1.0f;
   const int k = a.top_k ? a.top_k[b] : 0;
   // a vector as floats; NaN stays (it fails every comparison below)
   const auto floats = [&](const uint4 &v, float x[E]) {
@@ -445,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     // by weight alone those past x = -ln(V / (1 - p)) (together they weigh less than 1 - p of the first id, so top-p cuts
     // them whatever they are), and those that min-p leaves out, unless top-k's weight is top-p's whole
     float x_far = -INFINITY;
-    if (!by_count && p > 0.0f) x_far = -(logf((float)a.V) - logf(1.0f - p) + 0.1f);
+    if (!by_count && by_weight) x_far = -(logf((float)a.V) - logf(1.0f - p) + 0.1f);
     if (!(by_count && by_weight) && min_p > 0.0f) x_far = fmaxf(x_far, logf(fminf(min_p, 1.0f)) - 1e-3f);
     l_far = fminf(sc.lmax + x_far * T, nextafterf(sc.lmax, -INFINITY));
     float w = 0.0f, w_near = 0.0f;
