@@ -329,3 +329,17 @@ def test_no_top_p_leaves_the_first_id(V, bf16):
                   dict(m=nan), dict(k=300, m=nan), dict(T=nan), dict(T=nan, p=0.9)):
             tok, logp = _run(x, noise, **f)
             assert tok.tolist() == want and logp.tolist() == [0.0] * 3, (f, tok.tolist(), want)
+
+
+def test_infinity_ties_with_the_largest_float():
+    """+inf counts as the largest float: of the two the lower id comes first, within a thread's ids and between threads."""
+    import torch
+    big = float(np.finfo(np.float32).max)
+    for V, a, b in ((6, 0, 5), (6, 2, 3), (5000, 1, 4000), (5000, 6, 2048 + 6), (60000, 3, 59999)):
+        x = torch.zeros(2, V)
+        x[0, a], x[0, b] = big, math.inf
+        x[1, a], x[1, b] = math.inf, big
+        noise = torch.ones(2, V).cuda()
+        for f in (dict(T=0.0), dict(T=1.0), dict(k=1), dict(p=0.1), dict(k=2, p=0.4)):
+            tok, logp = _run(x.cuda(), noise, **f)
+            assert tok.tolist() == [a, a], (V, a, b, f, tok.tolist())

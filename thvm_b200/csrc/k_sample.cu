@@ -345,14 +345,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   int imax = 0;
 #pragma unroll 4
   for (int i = tid; i < nv; i += kThreads) {
-    const float x = largest(vector(i), In());
+    const float x = clean(largest(vector(i), In()));   // +inf ties with the largest float
     if (x > lmax) lmax = x, imax = i * E;   // i rises: the first vector that holds the largest
   }
   const auto raw = [&](int i) { return to_float(RESIDENT ? held[i] : __ldg(src + i)); };
   uint64_t top = 0;
   if (lmax > -INFINITY) {   // the first of the vector
     for (int e = E - 1; e >= 0; e--)
-      if (imax + e < n && raw(imax + e) == lmax) top = place(clean(lmax), begin + imax + e);
+      if (imax + e < n && clean(raw(imax + e)) == lmax) top = place(lmax, begin + imax + e);
   }
   top = block_max64(top, sh.red);
   if (tid == 0) sh.n_list = 0;
