@@ -2,6 +2,7 @@
 their contracts come back with a status and a message before anything touches
 a device."""
 import ctypes
+import math
 
 from thvm_b200 import _lib as L
 
@@ -124,3 +125,76 @@ def test_widest_workspace_is_that_of_eight_columns():
 
 def test_attention_refuses_a_scale_whose_logarithm_base_overflows():
     assert _attend(_cache(), scale=3e38) == L.ERR_ARG
+
+
+class FakePool:
+    """A pool or another tensor on cuda:1, as far as the calls look at one."""
+    is_cuda = True
+
+    def __init__(self, dtype, *shape):
+        import torch
+        self.dtype, self.shape, self.device = dtype, shape, torch.device("cuda", 1)
+        self.numel = lambda: math.prod(shape)
+        self.dim, self.is_contiguous, self.get_device, self.data_ptr = lambda: len(shape), lambda: True, lambda: 1, lambda: P
+        steps = [1]
+        for n in shape[:0:-1]:
+            steps.insert(0, steps[0] * n)
+        self.stride = lambda: tuple(steps)
+
+
+def test_calls_make_their_gpu_current(monkeypatch):
+    """A cache and a sampler on cuda:1 while cuda:0 is current: each call of the library runs with cuda:1 current, on its
+    stream, and cuda:0 is current again afterwards."""
+    import torch
+    from thvm_b200 import paged, sampling
+    current = [0]
+
+    class Guard:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0])
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 1000 + index)
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(paged.Scratch, "take", lambda self, n, device: self)
+    seen = []
+
+    def call(name):
+        return lambda *a: seen.append((name, current[0], a[-1] if a else None)) or 0
+
+    real, i32, f32, u8, bf16 = L.lib(), torch.int32, torch.float32, torch.uint8, torch.bfloat16
+    block = int(real.sm100_paged_block_bytes(16, 64, 16))
+
+    class Fake:
+        sm100_paged_block_bytes, sm100_paged_attention_ws_bytes = real.sm100_paged_block_bytes, real.sm100_paged_attention_ws_bytes
+        sm100_paged_append, sm100_paged_read, sm100_paged_attention = call("append"), call("read"), call("attend")
+        sm100_paged_status, sm100_sample = call("status"), call("sample")
+
+    monkeypatch.setattr(L, "lib", lambda: Fake)
+    monkeypatch.setattr(torch, "empty", lambda shape, dtype, device: FakePool(dtype, *(shape if isinstance(shape, tuple) else (shape,))))
+    FakePool.unbind = lambda self, d: (FakePool(self.dtype, *self.shape[1:]),) * 2
+    for here in (0, 1):
+        current[0] = here
+        c = paged.PagedCache(FakePool(u8, 4, 2, block), FakePool(i32, 2, 2), 16, 64, 16)
+        c.append(FakePool(f32, 2, 8 * 64), FakePool(i32, 2), FakePool(i32, 2), 4)
+        c.read(FakePool(i32, 2), FakePool(i32, 2))
+        c.attend(FakePool(bf16, 2, 4, 64), FakePool(i32, 2))
+        c.status()
+        s = sampling.Sampler(torch.device("cuda", 1))
+        s(FakePool(f32, 2, 8), FakePool(f32, 2, 8))
+        assert current[0] == here
+        assert seen == [("append", 1, 1001), ("read", 1, 1001), ("attend", 1, 1001), ("status", 1, None), ("sample", 1, 1001)]
+        seen.clear()
+
+
+def test_a_cache_is_on_a_gpu():
+    import pytest
+    from thvm_b200.paged import PagedCache
+    with pytest.raises(ValueError):
+        PagedCache.empty(2, 2, 4, 2, 64, device="cpu")

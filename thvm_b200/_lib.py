@@ -338,6 +338,21 @@ class Sm100Error(RuntimeError):
         self.code = code
 
 
+class OnDevice:
+    """Calls of the library with one GPU current: it launches on the current one,
+    and reads that one's status words, whatever the stream."""
+
+    def __init__(self, index: int):
+        import torch
+        self.index, self._current, self._guard = index, torch._C._cuda_getDevice, torch.cuda.device
+
+    def __call__(self, fn, *args):
+        if self._current() == self.index:
+            return fn(*args)
+        with self._guard(self.index):
+            return fn(*args)
+
+
 def check(code: int, what: str) -> int:
     if code != OK:
         raise Sm100Error(code, what)

@@ -8,8 +8,8 @@ cached rows as values.
     q = cache.append(qkv, pos, seq, heads=32, g_q=g_q, g_k=g_k, cos=cos, sin=sin)
     o = cache.attend(q, kv_len)
 
-PyTorch holds the memory; every call launches on torch's current stream and
-returns without waiting.  Calls on one PagedCache share its scratch, so they
+PyTorch holds the memory; every call launches on torch's current stream of the
+cache's GPU and returns without waiting.  Calls on one PagedCache share its scratch, so they
 belong on one stream; a cache given the `scratch` of another shares that too
 (the layers of a decoder need one between them).
 """
@@ -51,8 +51,10 @@ class PagedCache:
         block = int(self.lib.sm100_paged_block_bytes(page, head_dim, bits))
         if not block:
             raise ValueError(f"page {page} (16, 32, 64), head_dim {head_dim} (64, 128, 256), bits {bits} (4, 16)")
-        if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[2] != block or not pool.is_contiguous():
-            raise ValueError(f"pool must be uint8 [n_pages, kv_heads, {block}], got {pool.dtype} {tuple(pool.shape)}")
+        if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[2] != block or not pool.is_contiguous() or \
+                not pool.is_cuda:
+            raise ValueError(f"pool must be uint8 [n_pages, kv_heads, {block}] on a GPU, got {pool.dtype} "
+                             f"{tuple(pool.shape)} on {pool.device}")
         if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.device != pool.device:
             raise ValueError("table must be int32 [n_seq, max_pages] beside the pool")
         self.pool, self.table = pool, table
@@ -68,6 +70,7 @@ class PagedCache:
         self._rows = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16}
         self._append, self._read, self._attention = (
             self.lib.sm100_paged_append, self.lib.sm100_paged_read, self.lib.sm100_paged_attention)
+        self._on = L.OnDevice(self._index)
         self._need: dict[tuple[int, int], int] = {}
         # 8 query columns a unit are the widest layout
         self.scratch.take(int(self.lib.sm100_paged_attention_ws_bytes(self._desc, self.kv_heads, 8)), pool.device)
@@ -124,7 +127,7 @@ class PagedCache:
             qkv.data_ptr(), None if g_q is None else dense("g_q", g_q, f32, hd),
             None if g_k is None else dense("g_k", g_k, f32, hd), cos_ptr, sin_ptr, dense("pos", pos, i32, T),
             dense("seq", seq, i32, T), out_ptr, step if T > 1 else 0, T, heads, dtype, rot, n_pos, pairs, eps)
-        rc = self._append(self._desc, _addressof(a), self._raw_stream(self._index))
+        rc = self._on(self._append, self._desc, _addressof(a), self._raw_stream(self._index))
         if rc:
             L.check(rc, "paged_append")
         return out
@@ -135,8 +138,8 @@ class PagedCache:
         T = pos.numel()
         both = self._empty((2, T, self.kv_heads, self.head_dim), dtype=self._bf16, device=self._device)
         k, v = both.unbind(0)
-        rc = self._read(self._desc, self._dense("pos", pos, self._i32, T), self._dense("seq", seq, self._i32, T),
-                        k.data_ptr(), v.data_ptr(), T, self._raw_stream(self._index))
+        rc = self._on(self._read, self._desc, self._dense("pos", pos, self._i32, T), self._dense("seq", seq, self._i32, T),
+                      k.data_ptr(), v.data_ptr(), T, self._raw_stream(self._index))
         if rc:
             L.check(rc, "paged_read")
         return k, v
@@ -170,11 +173,11 @@ class PagedCache:
                                  None if q_off is None else dense("q_off", q_off, i32, self._n_seq + 1), out_ptr,
                                  ws.ptr, ws.nbytes, step if T > 1 else 0, T, heads, max_rows,
                                  hd ** -0.5 if scale is None else scale)
-        rc = self._attention(self._desc, _addressof(a), self._raw_stream(self._index))
+        rc = self._on(self._attention, self._desc, _addressof(a), self._raw_stream(self._index))
         if rc:
             L.check(rc, "paged_attention")
         return out
 
     def status(self) -> int:
         """Sticky error bits of the paged calls (0: none); waits for the GPU."""
-        return int(self.lib.sm100_paged_status())
+        return int(self._on(self.lib.sm100_paged_status))

@@ -23,6 +23,7 @@ class Sampler:
             self.device = torch.device("cuda", torch.cuda.current_device())
         # what every call looks up
         self._index, self._raw_stream, self._sample = self.device.index, torch._C._cuda_getCurrentRawStream, self.lib.sm100_sample
+        self._on = L.OnDevice(self._index)
         self._empty, self._f32, self._i32 = torch.empty, torch.float32, torch.int32
         self._rows = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16}
 
@@ -61,7 +62,7 @@ class Sampler:
             None if min_p is None else setting("min_p", min_p, f32, B),
             tok_ptr or setting("tok", tok, i32, B), logp_ptr or setting("logp", logp, f32, B),
             step if B > 1 else 0, noise_step if B > 1 else 0, B, V, dtype)
-        rc = self._sample(_addressof(a), self._raw_stream(self._index))
+        rc = self._on(self._sample, _addressof(a), self._raw_stream(self._index))
         if rc:
             L.check(rc, "sample")
         return tok, logp
