@@ -787,8 +787,8 @@ typedef struct Sm100PagedAttnArgs {
 } Sm100PagedAttnArgs;
 int sm100_paged_attention(const Sm100PagedCache *c, const Sm100PagedAttnArgs *a, void *stream);
 uint64_t sm100_paged_attention_ws_bytes(const Sm100PagedCache *c, int32_t heads, int32_t max_rows);
-/* the sticky status of the paged calls (SM100_DECODE_ERR_*); synchronises the
- * device and clears the word */
+/* the sticky status of the paged calls on the current device, whichever cache
+ * they were for (SM100_DECODE_ERR_*); synchronises the device and clears the word */
 uint32_t sm100_paged_status(void);
 
 /* ---- the next ids from logits ------------------------------------------------- */

@@ -706,3 +706,19 @@ def test_scale_zero_is_the_mean(bits, scale):
         assert bool(torch.isfinite(got).all())
         _check_attention(got, want, size)
         assert c.status() == 0
+
+
+def test_status_of_one_cache_is_not_taken_by_another():
+    import torch
+    from thvm_b200 import _lib as L
+    from thvm_b200.paged import PagedCache
+    a, b = (PagedCache.empty(1, 2, 2, 1, 64) for _ in range(2))
+    one = torch.zeros(1, dtype=torch.int32).cuda()
+    assert a.status() == b.status() == 0
+    a.read(one, one)                         # an empty slot of the table
+    assert b.status() == L.DECODE_ERR_ARG    # the GPU's word: b hears of it too,
+    assert a.status() == L.DECODE_ERR_ARG    # and a still does
+    assert a.status() == b.status() == 0
+    c = PagedCache.empty(1, 2, 2, 1, 64)
+    b.read(one, one)
+    assert a.status() == b.status() == c.status() == L.DECODE_ERR_ARG and c.status() == 0

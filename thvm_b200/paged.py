@@ -16,10 +16,12 @@ belong on one stream; a cache given the `scratch` of another shares that too
 from __future__ import annotations
 
 import ctypes
+import weakref
 
 from . import _lib as L
 
 _addressof = ctypes.addressof
+_caches: dict[int, weakref.WeakSet] = {}   # by GPU: who is to hear of its status word
 
 
 class Scratch:
@@ -71,6 +73,8 @@ class PagedCache:
         self._append, self._read, self._attention = (
             self.lib.sm100_paged_append, self.lib.sm100_paged_read, self.lib.sm100_paged_attention)
         self._on = L.OnDevice(self._index)
+        self._bits = 0   # of the status word, taken by another cache's status()
+        _caches.setdefault(self._index, weakref.WeakSet()).add(self)
         self._need: dict[tuple[int, int], int] = {}
         # 8 query columns a unit are the widest layout
         self.scratch.take(int(self.lib.sm100_paged_attention_ws_bytes(self._desc, self.kv_heads, 8)), pool.device)
@@ -179,5 +183,11 @@ class PagedCache:
         return out
 
     def status(self) -> int:
-        """Sticky error bits of the paged calls (0: none); waits for the GPU."""
-        return int(self._on(self.lib.sm100_paged_status))
+        """Error bits of the paged calls on this GPU since this cache last asked
+        (0: none); waits for the GPU.  The library has one word a GPU, which
+        reading clears: every cache hears of every bit, its own calls' or not."""
+        bits = int(self._on(self.lib.sm100_paged_status))
+        for c in list(_caches[self._index]):
+            c._bits |= bits
+        bits, self._bits = self._bits, 0
+        return bits

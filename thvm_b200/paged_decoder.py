@@ -210,5 +210,6 @@ class PagedDecoder:
         self.free_slots.append(s)
 
     def status(self) -> int:
-        """Sticky error bits of the pass's kernels (0: none); waits for the GPU."""
+        """Error bits of the pass's kernels on this GPU, other users' of them
+        included (0: none); waits for the GPU."""
         return self.cache[0].status() | int(self.lib.sm100_skinny_status()) << 16
