@@ -770,10 +770,12 @@ int sm100_paged_read(const Sm100PagedCache *c, const int32_t *pos, const int32_t
  * 0 .. kv_len[s] - n + r (kv_len counts the new tokens, appended before).  A
  * row that sees none (an idle sequence: kv_len 0), or only scores of -inf, is
  * zeros; a score of NaN or +inf makes the row's head NaN.  Tokens whose page
- * is outside the pool are left out and set the status word, as does a length
- * past max_pages * page (cut there).  scale 0 to 2e38.  q bf16, row stride ld_q elements (0:
- * dense), a multiple of 8; q, out, ws 16-byte aligned; heads / kv_heads whole.
- * ws: sm100_paged_attention_ws_bytes of scratch, zeroed before its first use and
+ * is outside the pool are left out and set the status word, as do a length past
+ * max_pages * page (cut there) or below 0 (taken as 0) and offsets that fall or
+ * lie outside 0 .. T (that sequence has no rows).  Rows that no sequence has are
+ * not written.  scale 0 to 2e38.  q bf16, row stride ld_q elements (0: dense), a
+ * multiple of 8; q, out, ws 16-byte aligned; heads / kv_heads whole.  ws:
+ * sm100_paged_attention_ws_bytes of scratch, zeroed before its first use and
  * left ready for the next call; calls that can overlap on the GPU need one
  * each. */
 typedef struct Sm100PagedAttnArgs {

@@ -722,3 +722,37 @@ def test_status_of_one_cache_is_not_taken_by_another():
     c = PagedCache.empty(1, 2, 2, 1, 64)
     b.read(one, one)
     assert a.status() == b.status() == c.status() == L.DECODE_ERR_ARG and c.status() == 0
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_rows_and_lengths_outside_set_the_status(bits):
+    """Offsets that fall or leave q, and lengths below 0: that sequence has no rows (no keys), the others are right, rows of no
+    sequence stay as they are, and the status says so."""
+    import torch
+    from thvm_b200 import _lib as L
+    rng = np.random.default_rng(51)
+    i = lambda *v: torch.tensor(v, dtype=torch.int32).cuda()
+    c = _cache([40, 20], 2, 64, 16, bits, rng)
+    _fill(c, [40, 20], rng)
+    q = torch.from_numpy(rng.standard_normal((4, 4, 64)).astype(np.float32)).cuda().bfloat16()
+    want, size = _attend_want(c, q, [40, 20], [2, 2], 0.125)
+    out = torch.empty_like(q)
+
+    def run(kv_len, q_off):
+        out.fill_(7.0)
+        c.attend(q, kv_len, q_off=q_off, max_rows=2, out=out)
+        return c.status()
+
+    assert run(i(40, 20), i(0, 2, 4)) == 0
+    _check_attention(out, want, size)
+    for q_off in (i(0, 2, 99), i(0, 2, 1), i(0, 2, -1), i(0, 2, 5)):
+        assert run(i(40, 20), q_off) == L.DECODE_ERR_ARG
+        _check_attention(out[:2], want[:2], size[:2])
+        assert bool((out[2:] == 7).all())
+    assert run(i(40, 20), i(-2, 0, 2)) == L.DECODE_ERR_ARG and bool((out[2:] == 7).all())
+    assert run(i(40, 20), i(9, 9, 9)) == L.DECODE_ERR_ARG and bool((out == 7).all())    # nothing to do, and past q
+    assert run(i(40, 20), i(1, 1, 1)) == 0 and bool((out == 7).all())
+    assert run(i(40, -3), i(0, 2, 4)) == L.DECODE_ERR_ARG
+    _check_attention(out[:2], want[:2], size[:2])
+    assert bool((out[2:] == 0).all())
+    assert run(i(40, -3), i(0, 0, 0)) == L.DECODE_ERR_ARG

@@ -173,12 +173,16 @@ struct Line {
   int tiles;                              // its tiles
   int64_t at;                             // its first place
 
-  __device__ __forceinline__ void load(int seq, int &r, int &f, int &l) const {
+  // false where something of it had to be left out
+  __device__ __forceinline__ bool load(int seq, int &r, int &f, int &l) const {
     f = a->q_off ? a->q_off[seq] : seq;
     r = a->q_off ? a->q_off[seq + 1] - f : 1;
     l = a->kv_len[seq];
-    if (f < 0 || r < 0 || f > a->T - r) r = 0;   // rows outside q: none
-    l = min(max(l, 0), c->max_pages * c->page);
+    const int most = c->max_pages * c->page;
+    const bool inside = f >= 0 && r >= 0 && f <= a->T - r, fits = l >= 0 && l <= most;
+    if (!inside) r = 0;   // rows outside q: none
+    l = min(max(l, 0), most);
+    return inside && fits;
   }
   __device__ __forceinline__ int columns(int r) const { return (r * a->group + NC - 1) / NC; }
   // token tiles up to the last key that a column tile's last row sees
@@ -308,7 +312,16 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
   const int me = blockIdx.x;
   int64_t total, w0, w1;
   int G, t0, t1;
-  if (!line.cut(gridDim.x, me, lane, total, G, w0, w1)) return;
+  const auto tell_bad_sequences = [&] {
+    for (int s = lane; s < c.n_seq; s += 32) {
+      int r, f, l;
+      if (!line.load(s, r, f, l)) atomicOr(&g_paged_status, SM100_DECODE_ERR_ARG);
+    }
+  };
+  if (!line.cut(gridDim.x, me, lane, total, G, w0, w1)) {
+    if (me == 0 && warp == NW) tell_bad_sequences();   // no rows at all
+    return;
+  }
   uint32_t it = 0;   // tiles through the ring
 
   if (warp == NW) {
@@ -350,10 +363,7 @@ __global__ void __launch_bounds__(Shape<HD, BITS, COLS>::NW * 32 + 32, Shape<HD,
       if (!ok_ring || line.at + kPad + line.tiles >= w1) break;
       line.next();
     }
-    if (me == 0) {   // lengths past the table were cut
-      for (int s = lane; s < c.n_seq; s += 32)
-        if (a.kv_len[s] > c.max_pages * c.page) atomicOr(&g_paged_status, SM100_DECODE_ERR_ARG);
-    }
+    if (me == 0) tell_bad_sequences();
     return;
   }
 

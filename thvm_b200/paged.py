@@ -152,7 +152,8 @@ class PagedCache:
         """softmax(q k^T scale) v of the new rows q (bf16 [T, heads, head_dim]),
         bf16 [T, heads, head_dim].  kv_len [n_seq] counts the cached tokens, the
         new ones among them; sequence s has the rows q_off[s] .. q_off[s + 1] - 1
-        (at most max_rows), without q_off row s alone (sm100_paged_attention)."""
+        (at most max_rows), without q_off row s alone; rows that no sequence has
+        are not written (sm100_paged_attention)."""
         hd, dense, i32 = self.head_dim, self._dense, self._i32
         T, heads, d = q.shape
         step, head, one = q.stride()
