@@ -198,3 +198,11 @@ def test_a_cache_is_on_a_gpu():
     from thvm_b200.paged import PagedCache
     with pytest.raises(ValueError):
         PagedCache.empty(2, 2, 4, 2, 64, device="cpu")
+
+
+def test_append_refuses_more_heads_than_it_can_count():
+    big = (1 << 31) - 2
+    assert _append(_cache(), heads=big) == L.ERR_ARG
+    assert _append(_cache(kv_heads=1 << 30), heads=1 << 30) == L.ERR_ARG
+    assert _append(_cache(kv_heads=1 << 30), heads=1 << 30, T=5) == L.ERR_ARG
+    assert _append(_cache(), heads=1 << 20, T=1 << 20) == L.ERR_ARG

@@ -344,7 +344,10 @@ extern "C" int sm100_paged_append(const Sm100PagedCache *c, const Sm100PagedAppe
                            a ? a->heads : 0, c->kv_heads);
   if (a->dtype != SM100_DT_F32 && a->dtype != SM100_DT_BF16)
     return sm100_set_error(SM100_ERR_UNSUPPORTED, "paged_append: qkv dtype %d (f32 or bf16)", a->dtype);
-  const int64_t width = ((int64_t)a->heads + 2 * c->kv_heads) * c->head_dim, ld = a->ld ? a->ld : width;
+  const int64_t n_heads = (int64_t)a->heads + 2 * (int64_t)c->kv_heads;
+  if (a->T * n_heads >= INT32_MAX)
+    return sm100_set_error(SM100_ERR_ARG, "paged_append: %d rows of %lld heads in one call", a->T, (long long)n_heads);
+  const int64_t width = n_heads * c->head_dim, ld = a->ld ? a->ld : width;
   const bool rot = a->cos_t || a->sin_t;
   if (rot && (!a->cos_t || !a->sin_t || a->rot < 16 || a->rot % 16 || a->rot > c->head_dim || a->n_pos < 1 ||
               !aligned16(a->cos_t) || !aligned16(a->sin_t)))
@@ -356,8 +359,6 @@ extern "C" int sm100_paged_append(const Sm100PagedCache *c, const Sm100PagedAppe
                            (long long)ld, (long long)width);
   AppendParams p{a->qkv, a->g_q, a->g_k, a->cos_t, a->sin_t, a->pos, a->seq, static_cast<__nv_bfloat16 *>(a->q_out),
                  ld, a->T, a->heads, rot ? a->rot : 0, a->n_pos, a->pairs, 0, 0, a->eps};
-  if ((int64_t)a->T * (a->heads + 2 * c->kv_heads) >= INT32_MAX)
-    return sm100_set_error(SM100_ERR_ARG, "paged_append: %d rows in one call", a->T);
   cudaStream_t st = (cudaStream_t)stream;
   const cudaError_t e = c->head_dim == 64    ? append_hd<64>(v, c->bits, a->dtype, p, st)
                         : c->head_dim == 128 ? append_hd<128>(v, c->bits, a->dtype, p, st)
