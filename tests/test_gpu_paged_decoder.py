@@ -165,3 +165,31 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         dec.admit([4])
     assert len(dec.step()) == 2 and dec.status() == 0
+
+
+def test_a_request_that_fails_or_fills_its_cache_leaves_the_others():
+    """A request that raises while it is admitted gives its slot and pages back; one that fills its cache is named, and the
+    others go on once it is released."""
+    from thvm_b200.paged_decoder import PagedConfig, PagedDecoder, paged_weights
+    cfg = PagedConfig(n_layers=1, dim=256, hidden=256, vocab=300, max_ctx=64)
+    w = paged_weights(cfg)
+    dec = PagedDecoder(cfg, w, n_seq=2, n_pages=8)
+    a = dec.admit([5, 6, 7], temperature=0.0)
+    state = (sorted(dec.free_pages), list(dec.free_slots), dict(dec.length), dict(dec.next_id))
+    for _ in range(3):   # more often than there are slots
+        with pytest.raises((TypeError, ValueError)):
+            dec.admit(range(20), top_k="many")
+        assert (sorted(dec.free_pages), list(dec.free_slots), dict(dec.length), dict(dec.next_id)) == state
+    b = dec.admit(range(63), temperature=0.0)
+    assert set(dec.step()) == {a, b}
+    before = (dict(dec.length), dict(dec.next_id))
+    with pytest.raises(RuntimeError, match=rf"\[{b}\]"):
+        dec.step()
+    assert (dict(dec.length), dict(dec.next_id)) == before
+    dec.release(b)
+
+    alone = PagedDecoder(cfg, w, n_seq=1, n_pages=8)
+    s = alone.admit([5, 6, 7], temperature=0.0)
+    want = [alone.step()[s] for _ in range(5)]
+    assert [before[1][a]] + [dec.step()[a] for _ in range(4)] == want
+    assert dec.status() == 0

@@ -17,7 +17,8 @@ then logits = bf16(rmsnorm(h)) W_lm^T and the next ids by Sampler.
     while ...: ids = dec.step()          # {s: next id}
     dec.release(s)
 
-PyTorch provides memory and copies; every kernel of a pass is the library's.
+PyTorch provides memory, copies and the random numbers; the kernels of a pass
+and of the draw are the library's.
 """
 from __future__ import annotations
 
@@ -182,17 +183,22 @@ class PagedDecoder:
             raise RuntimeError("no free page")
         s = self.free_slots.pop()
         self.pages[s], self.length[s], self.settings[s] = [], 0, (temperature, top_k, top_p, min_p)
-        for at in range(0, len(prompt), MAX_ROWS):
-            part = prompt[at:at + MAX_ROWS]
-            logits = self._pass([(s, part)])
-        self.next_id[s] = self._draw(logits[len(part) - 1:], [s])[0]
+        try:
+            for at in range(0, len(prompt), MAX_ROWS):
+                part = prompt[at:at + MAX_ROWS]
+                logits = self._pass([(s, part)])
+            self.next_id[s] = self._draw(logits[len(part) - 1:], [s])[0]
+        except BaseException:   # the request was not admitted: its slot and pages are free again
+            self.release(s)
+            raise
         return s
 
     def step(self) -> dict[int, int]:
         """Appends every request's last id and draws the next: {slot: id}."""
         slots = sorted(self.next_id)
-        if any(self.length[s] + 1 > self.cfg.max_ctx for s in slots):
-            raise RuntimeError("a request fills its cache: release it")
+        full = [s for s in slots if self.length[s] + 1 > self.cfg.max_ctx]
+        if full:   # nothing has changed: the others go on once these are released
+            raise RuntimeError(f"requests {full} fill their cache: release them")
         need = sum(self.length[s] % self.cfg.page == 0 for s in slots)
         if need > len(self.free_pages):
             raise RuntimeError("no free page")
@@ -205,9 +211,10 @@ class PagedDecoder:
     def release(self, s: int):
         """Ends a request: its pages and its slot are free."""
         self.free_pages += reversed(self.pages.pop(s))
-        self.table[s] = -1
-        del self.length[s], self.next_id[s], self.settings[s]
+        self.next_id.pop(s, None)
+        del self.length[s], self.settings[s]
         self.free_slots.append(s)
+        self.table[s] = -1
 
     def status(self) -> int:
         """Error bits of the pass's kernels on this GPU, other users' of them
