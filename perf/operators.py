@@ -30,8 +30,8 @@ GROUP = 64       # dimensions that share a scale and a minimum
 EPS = 1e-6
 TABLE = 40960    # rows of the rotation tables
 
-# (query heads, key / value heads, head dimension): the framework's own decoders (12 and 25 heads of 64, 16 of 128)
-# and grouped layouts
+# (query heads, key / value heads, head dimension): the head layouts of the framework's decoders (12 and 25 heads of 64,
+# 16 of 128), which keep their caches in fixed slots so far, and grouped ones as PagedDecoder's
 HEADS = [(12, 12, 64), (25, 25, 64), (16, 16, 128), (32, 8, 128), (28, 4, 128), (64, 8, 128), (8, 1, 128), (16, 2, 256)]
 
 
@@ -95,7 +95,7 @@ def draw(rng):
         else:
             case = dict(op=op, rows=_log(rng, 1, 256), vocab=_log(rng, 1000, 131072), bf16=rng.random() < 0.5,
                         kind=rng.choice(["topk", "topp", "mixed", "none"]), masked=rng.random() < 0.3)
-        if _size(case) <= most and 3072 not in case.values():
+        if _size(case) <= most and 3072 not in case.values():  # a size that no configuration here has stays out
             return case
 
 
@@ -430,7 +430,8 @@ def exact(case, seed):
             y = t.reshape(*t.shape[:-1], hd // GROUP, GROUP)
             lo, hi = y.min(-1, keepdim=True).values, y.max(-1, keepdim=True).values
             step, base = ((hi - lo) / 15).to(torch.bfloat16).to(f), lo.to(torch.bfloat16).to(f)
-            return (base + step * torch.clamp(torch.round((y - base) / step), 0, 15)).reshape(t.shape)
+            code = torch.where(step > 0, torch.clamp(torch.round((y - base) / step), 0, 15), 0.0)  # equal values: their minimum
+            return (base + step * code).reshape(t.shape)
 
         return dict(q=parts[0], k=held(k), v=held(v))
     out, at, G = [], 0, H // kv
