@@ -62,14 +62,19 @@ struct AttnParams {
   const __nv_bfloat16 *q;
   const int32_t *kv_len, *q_off;
   __nv_bfloat16 *out;
-  float *parts;        // [gridDim][2] of kPart floats
+  float *parts;        // [gridDim][2] of Shape::PART floats
   uint32_t *counters;  // [gridDim], zero between launches
   int64_t ld_q;
   int T, heads, group;
   float scale_log2;    // scale * log2(e)
 };
 
-constexpr int kMaxPieces = 148 * 4;   // CTAs of a launch at most
+constexpr int kSMs = 148;
+
+// CTAs of an SM: what the registers leave (5 warps each: 128 registers at 3, 168 at 2, 255 at 1)
+constexpr int ctas_of(int hd, int bits) { return hd == 256 ? (bits == 4 ? 2 : 1) : hd == 128 && bits == 16 ? 2 : 3; }
+
+constexpr int kCounters = kSMs * 4;   // the most CTAs of a launch are 3 an SM
 
 // COLS query columns a unit: 4 (4 bits only: the weights' low parts take the
 // other half of the 8 columns of a product) or 8.  Two products a unit, 16
@@ -91,12 +96,12 @@ struct Shape {
   static constexpr int CHUNK = 4;                               // of them joined at a time, one a warp
   static constexpr int PART = ACC * 128 + 2 * COLS;             // floats of a unit's part
   static constexpr int RED = NW * CHUNK * 512;
-  // CTAs of an SM: what the registers leave (5 warps each: 128 registers at 3, 168 at 2)
-  static constexpr int CTAS = HD == 256 ? (BITS == 4 ? 2 : 1) : HD == 128 && BITS == 16 ? 2 : 3;
+  static constexpr int CTAS = ctas_of(HD, BITS);
   static constexpr int ROOM = 227 * 1024 / CTAS - RED - 3072;
   static constexpr int STAGES = ROOM / TILE > 8 ? 8 : ROOM / TILE;
   static constexpr int SMEM = STAGES * TILE + RED;
   static_assert(STAGES >= 2, "a ring needs two stages");
+  static_assert(CTAS * kSMs <= kCounters, "a counter a CTA");
 };
 
 __device__ __forceinline__ void mma_bf16(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
@@ -821,10 +826,11 @@ int launch(const PagedView &v, AttnParams &p, const Sm100PagedAttnArgs *a, cudaS
         (e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, S::NW * 32 + 32, S::SMEM)) != cudaSuccess)
       return sm100_set_error(SM100_ERR_CUDA, "paged_attention: %s", cudaGetErrorString(e));
     if (per < 1) return sm100_set_error(SM100_ERR_UNSUPPORTED, "paged_attention: no room for %d bytes of shared memory", S::SMEM);
-    grid[dev] = sms * per < kMaxPieces ? sms * per : kMaxPieces;
+    const int most = kSMs * S::CTAS;   // what the scratch holds parts for
+    grid[dev] = sms * per < most ? sms * per : most;
   }
   p.counters = static_cast<uint32_t *>(a->ws);
-  p.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(a->ws) + kMaxPieces * 4);
+  p.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(a->ws) + kCounters * 4);
   e = launch_pdl(kernel, dim3(grid[dev]), dim3(S::NW * 32 + 32), S::SMEM, st, v, p);
   if (e != cudaSuccess) return sm100_set_error(SM100_ERR_CUDA, "paged_attention: %s", cudaGetErrorString(e));
   return launch_status("paged_attention");
@@ -847,7 +853,7 @@ extern "C" uint64_t sm100_paged_attention_ws_bytes(const Sm100PagedCache *c, int
   PagedView v;
   if (sm100_paged_view(c, "paged_attention_ws_bytes", &v) || heads < 1 || heads % c->kv_heads || max_rows < 1) return 0;
   const uint64_t cols = columns_of(c->bits, (int64_t)max_rows * (heads / c->kv_heads));
-  return kMaxPieces * 4 + (uint64_t)kMaxPieces * 2 * (8 * c->head_dim + 2 * cols) * 4;
+  return kCounters * 4 + (uint64_t)kSMs * ctas_of(c->head_dim, c->bits) * 2 * (8 * c->head_dim + 2 * cols) * 4;
 }
 
 extern "C" int sm100_paged_attention(const Sm100PagedCache *c, const Sm100PagedAttnArgs *a, void *stream) {
