@@ -743,11 +743,11 @@ uint64_t sm100_paged_block_bytes(int32_t page, int32_t head_dim, int32_t bits); 
  * head are rotated by row pos[t] (pair i: dimensions i and i + rot / 2, or
  * with pairs != 0 dimensions 2 i and 2 i + 1); queries go to q_out (bf16 [T]
  * [heads][head_dim]), keys and values into the cache.  All in f32, rounded
- * once (Q4: to codes of the group's bf16 scale = (max - min) / 15 and minimum;
- * a group with a value that is not finite reads as NaN).  A row whose
- * sequence, position or page is outside the cache or the tables is skipped:
- * its queries are zeros and sm100_paged_status gets SM100_DECODE_ERR_ARG.  No
- * two rows of a call may be the same token.  qkv, q_out 16-byte aligned, ld a
+ * once (Q4: to codes of the group's bf16 minimum and scale, (max - min) times the
+ * f32 nearest to 1 / 15; a group with a value that is not finite, or whose scale
+ * is not, reads as NaN).  A row whose sequence, position or page is outside the
+ * cache or the tables is skipped: its queries are zeros and sm100_paged_status
+ * gets SM100_DECODE_ERR_ARG.  No two rows of a call may be the same token.  qkv, q_out 16-byte aligned, ld a
  * multiple of 8 (bf16) or 4 (f32), rot a multiple of 16. */
 typedef struct Sm100PagedAppendArgs {
   const void *qkv;
@@ -807,8 +807,11 @@ uint32_t sm100_paged_status(void);
  * are left out, +inf counts as the largest float; a row with none left gives id
  * -1 and logp -inf.  temperature, top_k,
  * top_p, min_p: device arrays [B], or NULL (1, all, all, all).  V < 2^23.  The
- * weights of the filters are summed exactly in units of 2^-40: the cut does
- * not depend on an order of summation. */
+ * weights of up to V / 512 ids are summed in f32 at first (off by 2^-33 V of the
+ * sum at most, some 2^-24 as a rule), and these sums exactly: the same call gives
+ * the same bits each time, but which ids are summed together follows from B and V,
+ * so an id whose forerunners hold top_p of the weight to within that error
+ * may be kept in one batch and not in another. */
 typedef struct Sm100SampleArgs {
   const void *logits;
   const float *noise, *temperature;

@@ -5,8 +5,9 @@
 // Per head x[hd] of a row at position p: y = x * rsqrt(sum x^2 / hd + eps) * g
 // (queries and keys, where there is a g); (y_a, y_b) -> (y_a cos - y_b sin,
 // y_b cos + y_a sin) over the rotated pairs; then one rounding: bf16, or per 64
-// dimensions m = bf16(min), s = bf16((max - min) / 15), code = round((y - m) /
-// s) clamped to 0..15.  The codes are taken against the rounded m and s, so
+// dimensions m = bf16(min), s = bf16((max - min) * r), r = 1 / 15 rounded to f32
+// (a product in place of a division; the two differ where (max - min) / 15 lies
+// within 2^-23 of it from a tie of bf16), code = round((y - m) / s) clamped to 0..15.  The codes are taken against the rounded m and s, so
 // their rounding does not add to the value's error except at the ends.
 //
 // A thread holds 8 neighbouring dimensions in f32 (one 16-byte load of bf16,
@@ -90,11 +91,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 __device__ __forceinline__ float shfl_add(float v, int o) { return __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, o)); }
 
-// sum x^2 of a head in one fixed order that does not depend on how the head is
-// spread over lanes, each step rounded on its own: squares are added up in
-// runs of `unit` neighbours (256 dimensions: the two halves first), then by
-// halves, element i with element i + n / 2.  A key that a plain evaluation of
-// the formula in this order quantises gets the same codes here, ties included.
+// sum x^2 of a head in one fixed order for each head size, each step rounded on
+// its own: 256 dimensions add their two halves, 128 add up runs of 4 neighbours,
+// and what there is adds its halves, element i with i + n / 2, until one is left.
+// There is no numerical reason for these orders, and they are not the cheapest:
+// the formula written in torch operations is summed like this on this GPU, and a
+// key gets the code here that it gets there, ties between two codes included.
 template <int HD>
 __device__ __forceinline__ float sum_squares(const float x[8]) {
   float s[8];

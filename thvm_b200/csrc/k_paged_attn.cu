@@ -6,10 +6,10 @@
 // (the heads of a group times the new rows), so a decode step is bound by
 // memory: bf16 pages stream at 5.5 TB/s (16 sequences of 4096, 8 key heads of
 // 128: 49 us).  In 4 bits, where a token of 128 + 128 dimensions is 144 bytes,
-// issue and the integer pipe bind first: of the 365 instructions for 16 tokens
-// 137 are the shifts and ANDs that unpack (16 sequences of 16384: 57 % of the
+// issue and the integer pipe bind first: of the 369 instructions for 16 tokens
+// 136 are the shifts and ANDs that unpack (16 sequences of 16384: 57 % of the
 // issue slots and 58 % of the integer pipe, memory at 42 %; 64 of up to 16384:
-// 139 us, 3.8 TB/s).  Short calls are bound by the chain lengths -> cut -> table
+// 137 us, 3.8 TB/s).  Short calls are bound by the chain lengths -> cut -> table
 // -> first tile and by the joining (one sequence of 32768 in 4 bits, 24 us: tiles
 // done after 7 to 15, the last unit joined 10 later).
 //
@@ -167,7 +167,8 @@ __device__ __forceinline__ uint32_t codes31(uint32_t w, int i) {
 // places for what a unit costs beside its tiles (queries, joining, output:
 // about that many tiles' time), then its token tiles.  1, 2, 3, 4 places: 64
 // sequences of up to 16384 take 145, 138, 139, 140 us, 8 of up to 4096 with 4 new
-// rows 34.8, 34.1, 35.5, 36.4.
+// rows 34.8, 34.1, 35.5, 36.4: in these two 1 is too few, and 2 to 4 are within 1 and
+// 7 % of each other.
 constexpr int kPad = 2;
 
 template <int TS, int NC>

@@ -13,11 +13,11 @@
 // is a Gumbel number, so id i wins with probability w_i / sum w.
 //
 // What bounds it: the logits once (and the random numbers of the kept ids) is the
-// floor; above it, with many rows the slowest row (256 x 102400 bf16: 79 to 88 us
-// with the draw of the settings, 8 for the bytes, 32 instructions an id over all
+// floor; above it, with many rows the slowest row (256 x 102400 bf16: 79 to 93 us
+// with the draw of the settings, 8 for the bytes, 33 instructions an id over all
 // passes; a traced row takes 35 us on average, the longest 66), with few rows the
-// latency of the steps one after the other (one row of 50257: 16 us, 32 of 102400:
-// 30 to 32).  A row belongs to one CTA, or with few rows to a cluster of 2 to 8
+// latency of the steps one after the other (one row of 50257: 17 us, 32 of 102400:
+// 30 to 33).  A row belongs to one CTA, or with few rows to a cluster of 2 to 8
 // that holds it in shared memory where it fits (later passes come from L2
 // otherwise).  A cut is found without sorting the row:
 //   1. a histogram of (l_max - l) / T in 4096 bins of 1/128 of the ids that can
@@ -32,10 +32,15 @@
 // Where everything above the cut fits in the list too (top-k of up to some
 // hundreds, a peaked top-p) the list is all that is kept, and CTA 0 runs the
 // race on it alone.  A bin that overflows the list (thousands of equal logits at
-// the cut) falls back to a bisection over the 64 bits of a place.
-// A thread sums the weights of its few dozen ids in f32, in a fixed order; from
-// there on sums are 64-bit integers in units of 2^-40, so no order of arrival
-// enters a result.
+// the cut) falls back to a bisection over the 64 bits of a place, a pass over the
+// row for each: rows of one value take 185 to 200 us at 1 x 50257, 3.5 to 5.7 ms at 256
+// x 102400.
+// A thread sums the weights of its ids in f32, in a fixed order (V / 512 of them
+// where one CTA has the row, 200 at 102400, fewer with more CTAs); from there on
+// sums are 64-bit integers in units of 2^-40, so no order of arrival enters a
+// result.  What a thread sums depends on the CTAs a row, and so on the batch: the
+// totals of a row with 1, 2, 4 and 8 differ by some 2e-8 of it (emulated).  Whole
+// numbers for every id would cost a conversion each, some 8 us when it was tried.
 #include "common.cuh"
 #include "sample_bins.h"
 
