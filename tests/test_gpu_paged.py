@@ -606,9 +606,11 @@ def test_weights_keep_sixteen_bits(bits, H):
     assert bool((err <= 2.0 ** -8 * want.abs() + 2.0 ** -15 * size).all()), float((err / size).max())
 
 
-def test_graph_stays_right_after_wider_eager_calls():
-    """A decode step in 4 bits captured as the cache's first attention (4 query columns a unit), then a part of a prompt and
-    verify rows eagerly, memory taken and filled by others, and replays: the graph's results and the others' memory hold."""
+@pytest.mark.parametrize("warm", [True, False])
+def test_graph_stays_right_after_wider_eager_calls(warm):
+    """A decode step in 4 bits (4 query columns a unit), eagerly first or not, is captured; then a part of a prompt and verify
+    rows run eagerly, others take memory and fill it, and the graph is replayed between eager calls: the graph's results,
+    theirs and the others' memory hold."""
     import torch
     rng = np.random.default_rng(41)
     H, kv, hd, page, n = 8, 2, 128, 64, 6000    # units cut between CTAs: parts and counters are used
@@ -617,25 +619,26 @@ def test_graph_stays_right_after_wider_eager_calls():
     q = torch.from_numpy(rng.standard_normal((33, H, hd)).astype(np.float32)).cuda().bfloat16()
     kv_len = torch.tensor([n], dtype=torch.int32).cuda()
     o = torch.empty(1, H, hd, dtype=torch.bfloat16, device="cuda")
+    if warm:
+        c.attend(q[:1], kv_len, out=o)
+    at = c.scratch.ptr
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         c.attend(q[:1], kv_len, out=o)
-    at = c.scratch.ptr
-    for rows in (33, 4):
+        c.attend(q[:1], kv_len, out=o)
+    for rows in (33, 4):    # before the first replay
         want, size = _attend_want(c, q[:rows], [n], [rows], hd ** -0.5)
         got = c.attend(q[:rows], kv_len, q_off=torch.tensor([0, rows], dtype=torch.int32).cuda(), max_rows=rows)
         _check_attention(got, want, size)
-    assert c.scratch.ptr == at
+    assert c.scratch.ptr == at or not warm
     others = [torch.full((1 << 20,), 7, dtype=torch.int32, device="cuda") for _ in range(16)]
     want, size = _attend_want(c, q[:1], [n], [1], hd ** -0.5)
     for _ in range(3):
         o.zero_()
         g.replay()
         _check_attention(o, want, size)
+        _check_attention(c.attend(q[:1], kv_len), want, size)
     assert all(bool((t == 7).all()) for t in others)
-    with pytest.raises(RuntimeError):   # a cache made inside a capture would have its workspace zeroed by replays alone
-        with torch.cuda.graph(torch.cuda.CUDAGraph()):
-            type(c)(c.pool, c.table, page, hd, 4)
     assert c.status() == 0
 
 

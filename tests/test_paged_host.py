@@ -102,16 +102,20 @@ def test_scratch_keeps_what_a_graph_may_hold(monkeypatch):
     cpu, capturing = torch.device("cpu"), []
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: bool(capturing))
     s = Scratch()
-    small = s.take(64, cpu).ptr
-    assert s.take(32, cpu).ptr == s.take(64, cpu).ptr == small   # large enough: it stays where it is
-    assert s.take(128, cpu).ptr != small and s.nbytes == 128
-    assert [b.data_ptr() for b in s.held] == [small, s.ptr]      # the earlier memory is no one else's
+    small = s.take(64, cpu)[0]
+    assert s.take(32, cpu) == s.take(64, cpu) == (small, 64)     # large enough: it stays where it is
+    large = s.take(128, cpu)[0]
+    assert large != small and s.take(1, cpu) == (large, 128)
+    assert [b.data_ptr() for b in s.held] == [small, large]      # the earlier memory is no one else's
     with pytest.raises(ValueError):
         s.take(16, torch.device("cuda", 0))
     capturing.append(True)
-    assert s.take(128, cpu).nbytes == 128
-    with pytest.raises(RuntimeError):
-        s.take(129, cpu)
+    assert s.take(128, cpu) == (large, 128)
+    graph = s.take(129, cpu)                                     # zeroed by replays: the graph's alone
+    assert graph[1] == 129 and graph[0] not in (small, large) and s.held[-1].data_ptr() == graph[0]
+    capturing.clear()
+    assert s.take(128, cpu) == (large, 128)
+    assert s.take(129, cpu)[0] not in (small, large, graph[0])
 
 
 def test_widest_workspace_is_that_of_eight_columns():
@@ -162,7 +166,7 @@ def test_calls_make_their_gpu_current(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0])
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 1000 + index)
     monkeypatch.setattr(torch.cuda, "device", Guard)
-    monkeypatch.setattr(paged.Scratch, "take", lambda self, n, device: self)
+    monkeypatch.setattr(paged.Scratch, "take", lambda self, n, device: (P, n))
     seen = []
 
     def call(name):

@@ -25,23 +25,26 @@ _caches: dict[int, weakref.WeakSet] = {}   # by GPU: who is to hear of its statu
 
 
 class Scratch:
-    """The attention's workspace.  A cache takes what its widest call needs when
-    it is made, so no call moves it; where a cache of wider heads joins later,
-    the earlier memory is kept, since a captured graph may hold its address."""
+    """The attention's workspace.  A cache's first attention takes what its widest
+    call needs, so no later one moves it.  No memory is given back, since a
+    captured graph may hold its address: neither what a cache of wider heads
+    outgrows, nor what a first attention under capture takes, which is zeroed by
+    the graph's replays alone and so stays with the graph."""
 
     def __init__(self):
         self.held, self.ptr, self.nbytes = [], 0, 0
 
-    def take(self, nbytes: int, device):
+    def take(self, nbytes: int, device) -> tuple[int, int]:
+        """(address, bytes) of a workspace of nbytes or more."""
         import torch
         if self.held and self.held[-1].device != device:
             raise ValueError(f"a scratch on {self.held[-1].device} for a cache on {device}")
         if nbytes > self.nbytes:
-            if torch.cuda.is_current_stream_capturing():   # the zeros would be written by the replays alone
-                raise RuntimeError("the attention's workspace cannot be made while a graph is captured")
             self.held.append(torch.zeros(nbytes, dtype=torch.uint8, device=device))   # counters start at zero
+            if torch.cuda.is_current_stream_capturing():
+                return self.held[-1].data_ptr(), nbytes
             self.ptr, self.nbytes = self.held[-1].data_ptr(), nbytes
-        return self
+        return self.ptr, self.nbytes
 
 
 class PagedCache:
@@ -77,7 +80,7 @@ class PagedCache:
         _caches.setdefault(self._index, weakref.WeakSet()).add(self)
         self._need: dict[tuple[int, int], int] = {}
         # 8 query columns a unit are the widest layout
-        self.scratch.take(int(self.lib.sm100_paged_attention_ws_bytes(self._desc, self.kv_heads, 8)), pool.device)
+        self._widest = int(self.lib.sm100_paged_attention_ws_bytes(self._desc, self.kv_heads, 8))
 
     @classmethod
     def empty(cls, n_seq: int, max_pages: int, n_pages: int, kv_heads: int, head_dim: int, page: int = 32,
@@ -173,10 +176,12 @@ class PagedCache:
             if not need:
                 raise ValueError(f"heads {heads} (a multiple of {self.kv_heads}), max_rows {max_rows}")
             self._need[heads, max_rows] = need
-        ws = self.scratch
+        ws, ws_bytes = self.scratch.ptr, self.scratch.nbytes
+        if ws_bytes < self._widest:
+            ws, ws_bytes = self._on(self.scratch.take, self._widest, self._device)
         a = L.Sm100PagedAttnArgs(q.data_ptr(), dense("kv_len", kv_len, i32, self._n_seq),
                                  None if q_off is None else dense("q_off", q_off, i32, self._n_seq + 1), out_ptr,
-                                 ws.ptr, ws.nbytes, step if T > 1 else 0, T, heads, max_rows,
+                                 ws, ws_bytes, step if T > 1 else 0, T, heads, max_rows,
                                  hd ** -0.5 if scale is None else scale)
         rc = self._on(self._attention, self._desc, _addressof(a), self._raw_stream(self._index))
         if rc:
