@@ -343,3 +343,37 @@ def test_infinity_ties_with_the_largest_float():
         for f in (dict(T=0.0), dict(T=1.0), dict(k=1), dict(p=0.1), dict(k=2, p=0.4)):
             tok, logp = _run(x.cuda(), noise, **f)
             assert tok.tolist() == [a, a], (V, a, b, f, tok.tolist())
+
+
+@pytest.mark.parametrize("V", [61, 3000, 40001])
+@pytest.mark.parametrize("base", [1e4, -3e3, 700.0])
+def test_min_p_at_low_temperatures_beside_large_logits(V, base):
+    """Logits whose spacing in f32 is near the temperature: what min-p keeps is every id whose weight reaches it.
+
+    l - l_max is exact here (neighbours of one size), so w is good to |d| 2^-23 and 2^-22; an id within 1e-5 of the bound is not
+    asked for.  As above, the id with a random number of nearly nothing is chosen exactly where it is kept."""
+    import torch
+    rng = np.random.default_rng(V)
+    step = float(np.spacing(np.float32(abs(base))))
+    row = (np.float32(base) - np.float32(step) * rng.integers(0, 40, V).astype(np.float32)).astype(np.float32)
+    for spread in (0.05, 0.31, 0.9, 1.7):
+        T = np.float32(step / spread)
+        order, d = _kept(row.astype(np.float64), np.float64(T), None, None, None)
+        w = np.exp(d)
+        before = np.cumsum(w) - w
+        for m in (1e-6, 0.02, 0.3, 0.7):
+            for extra in (dict(), dict(k=V - 1), dict(p=0.99), dict(p=0.9999)):
+                p = np.float64(np.float32(extra.get("p", 1.0)))
+                kept = (w >= np.float64(np.float32(m))) & (before < p * w.sum()) & (np.arange(V) < extra.get("k", V))
+                sure = (np.abs(w / np.float64(np.float32(m)) - 1) > 1e-5) & (np.abs(before / w.sum() - p) > 1e-5)
+                n = int(kept.sum())   # a beginning of the order
+                ends = np.append(np.flatnonzero(np.diff(d) < 0), V - 1)   # the last id of each level
+                asked = [i for i in sorted({0, 1, n // 2, n - 2, n - 1, n, n + 1, *ends.tolist()})
+                         if 0 <= i < V and sure[i] and i < 4 * n + 50][:24]
+                ids = order[asked]
+                noise = torch.ones(len(ids), V, device="cuda")
+                noise[torch.arange(len(ids)), torch.from_numpy(ids.copy()).cuda()] = 1e-38
+                x = torch.from_numpy(row).cuda().expand(len(ids), V).contiguous()
+                tok, _ = _run(x, noise, T=float(T), m=m, **extra)
+                want = np.where(np.array(asked) < n, ids, order[0])
+                assert (tok.cpu().numpy() == want).all(), (V, base, spread, m, extra, n, asked)

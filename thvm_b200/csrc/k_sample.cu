@@ -451,7 +451,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     float x_far = -INFINITY;
     if (!by_count && by_weight) x_far = -(logf((float)a.V) - logf(1.0f - p) + 0.1f);
     if (!(by_count && by_weight) && min_p > 0.0f) x_far = fmaxf(x_far, logf(fminf(min_p, 1.0f)) - 1e-3f);
-    l_far = fminf(sc.lmax + x_far * T, nextafterf(sc.lmax, -INFINITY));
+    // (the last term: more than the roundings of the others, which are many nats where T is small beside l_max)
+    const float below = x_far * T;
+    l_far = fminf(sc.lmax + below - 0x1p-22f * (fabsf(sc.lmax) - below), nextafterf(sc.lmax, -INFINITY));
     float w = 0.0f, w_near = 0.0f;
     each_vector([&](const uint4 &v, int) {
       float x[E];
