@@ -9,7 +9,7 @@
 // issue and the integer pipe bind first: of the 369 instructions for 16 tokens
 // 136 are the shifts and ANDs that unpack (16 sequences of 16384: 57 % of the
 // issue slots and 58 % of the integer pipe, memory at 42 %; 64 of up to 16384:
-// 137 us, 3.8 TB/s).  Short calls are bound by the chain lengths -> cut -> table
+// 137 to 141 us, 3.8 TB/s).  Short calls are bound by the chain lengths -> cut -> table
 // -> first tile and by the joining (one sequence of 32768 in 4 bits, 24 us: tiles
 // done after 7 to 15, the last unit joined 10 later).
 //

@@ -17,7 +17,7 @@
 // with the draw of the settings, 8 for the bytes, 33 instructions an id over all
 // passes; a traced row takes 35 us on average, the longest 66), with few rows the
 // latency of the steps one after the other (one row of 50257: 17 us, 32 of 102400:
-// 30 to 33).  A row belongs to one CTA, or with few rows to a cluster of 2 to 8
+// 30 to 34).  A row belongs to one CTA, or with few rows to a cluster of 2 to 8
 // that holds it in shared memory where it fits (later passes come from L2
 // otherwise).  A cut is found without sorting the row:
 //   1. a histogram of (l_max - l) / T in 4096 bins of 1/128 of the ids that can
